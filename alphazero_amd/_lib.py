@@ -119,6 +119,13 @@ SIGNATURES = {
     "az_tower_flops_per_eval": (C.c_double, [_P]),
     "az_tower_conv_kernel": (C.c_char_p, [_P]),
     "az_search_run": (_I, [_P, _I]),
+    "az_layer_norm_fwd_dev": (_I, [_I, _P, _I, _I, C.c_int64, C.c_int64, C.c_double, _P, C.c_int64, _P, _P, _P, C.c_int64, _P, _P]),
+    "az_layer_norm_bwd_workspace": (C.c_int64, [C.c_int64, C.c_int64]),
+    "az_layer_norm_bwd_dev": (_I, [_I, _P, _I, _I, C.c_int64, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, _P, _P, C.c_int64,
+                                   _P, _P, _P, C.c_int64]),
+    "az_adamw_step_dev": (_I, [_I, _P, C.c_int64, _P, _P, _P, _P, _P, _P, _P, _I, C.c_double, C.c_double, C.c_double, C.c_double,
+                               C.c_double, C.c_int64]),
+    "az_dequantize_state_dev": (_I, [_I, _P, _P, _P, C.c_int64, _I, _P]),
     "az_tower_profile": (_I, [_P, _I]),
     "az_tower_leaf_compaction": (_I, [_P, _I]),
     "az_counters_get": (_I, [_P, C.POINTER(AzCounters)]),
@@ -137,6 +144,12 @@ def lib():
             raise ImportError(
                 "alphazero_amd: %s is missing - build it with `python -c 'import __graft_entry__ as g; g.build()'` "
                 "or `make -C alphazero_amd/csrc`" % LIB_PATH)
+        try:
+            # PyTorch brings a HIP runtime of its own; loaded first, it serves this library too, and streams can be handed
+            # from one to the other.  Loaded second there would be two runtimes in the process.
+            import torch  # noqa: F401
+        except ImportError:
+            pass
         L = C.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(L, name)

@@ -2,6 +2,7 @@
 #include "../../include/az_engine.h"
 #include "az_kernels.h"
 #include "az_tower.h"
+#include "az_error.h"
 
 #include <algorithm>
 #include <cstdio>
@@ -10,8 +11,13 @@
 #include <string>
 #include <vector>
 
-// why the last az_engine_create of the calling thread failed (there is no handle to hang the message on)
+// why the last az_engine_create, or call without a handle, of the calling thread failed (there is no handle to hang the message on)
 static thread_local std::string g_create_error;
+int az_fail(int code, const char *message) noexcept
+{
+    try { g_create_error = message; } catch (...) {}   // (out of host memory: the code alone has to do)
+    return code;
+}
 #define AZ_EVQ 8
 
 // Staging of az_trajectory_pop_many_static: a fixed array in every GPU's memory instead of a buffer grown with

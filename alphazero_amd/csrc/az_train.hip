@@ -1,0 +1,294 @@
+// Training operators of the C ABI (include/az_engine.h): layer norm with its gradient, the AdamW step.
+#include "../../include/az_engine.h"
+#include "az_error.h"
+#include "az_norm_kernels.h"
+#include "az_adamw_kernels.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <vector>
+
+namespace {
+
+// The caller's device for the duration of a call: kernels go to the device of the tensors, the calling thread's current
+// device stays what it was.
+struct DeviceScope {
+    int before = -1, now;
+    hipError_t error;
+    explicit DeviceScope(int device) : now(device)
+    {
+        error = hipGetDevice(&before);
+        if (error == hipSuccess && before != device) error = hipSetDevice(device);
+    }
+    ~DeviceScope() { if (before >= 0 && before != now) (void)hipSetDevice(before); }
+};
+
+int fail_hip(const char *what, hipError_t e)
+{
+    char buf[256];
+    snprintf(buf, sizeof buf, "%s: %s", what, hipGetErrorString(e));
+    return az_fail(AZ_ERR_HIP, buf);
+}
+
+// Workgroups that keep the chip's memory busy when each walks over many rows: eight of 256 threads fit a compute unit at once.
+int64_t resident_blocks() { return 256 * 8; }
+
+bool bad_type(int32_t t) { return t != AZ_TYPE_F32 && t != AZ_TYPE_BF16 && t != AZ_TYPE_F16; }
+
+// threads per row and register groups per thread: the narrowest form that holds the row
+#define AZ_NORM_MAX_COLS 8192
+template <typename T, typename Launch> void norm_form(int64_t cols, const Launch &launch)
+{
+    if (cols <= 64) launch.template operator()<T, 16, 1>();
+    else if (cols <= 256) launch.template operator()<T, 64, 1>();
+    else if (cols <= 512) launch.template operator()<T, 64, 2>();
+    else if (cols <= 1024) launch.template operator()<T, 64, 4>();
+    else if (cols <= 2048) launch.template operator()<T, 256, 2>();
+    else if (cols <= 4096) launch.template operator()<T, 256, 4>();
+    else launch.template operator()<T, 256, 8>();
+}
+
+template <typename Launch> void by_type(int32_t type, const Launch &launch)
+{
+    if (type == AZ_TYPE_F32) launch.template operator()<float>();
+    else if (type == AZ_TYPE_BF16) launch.template operator()<__bf16>();
+    else launch.template operator()<_Float16>();
+}
+
+struct FwdForm {
+    const NormFwd &a; hipStream_t st;
+    template <typename T, int TPR, int NV> void operator()() const
+    {
+        const int64_t groups = AZ_NORM_THREADS / TPR, blocks = (a.rows + groups - 1) / groups;
+        k_layer_norm_fwd<T, TPR, NV><<<(unsigned)std::min(blocks, resident_blocks()), AZ_NORM_THREADS, 0, st>>>(a);
+    }
+};
+struct FwdType {
+    const NormFwd &a; hipStream_t st;
+    template <typename T> void operator()() const
+    {
+        if (a.cols > AZ_NORM_MAX_COLS) k_layer_norm_fwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2 * 256), AZ_NORM_WIDE_THREADS, 0, st>>>(a);
+        else norm_form<T>(a.cols, FwdForm{a, st});
+    }
+};
+
+// Workgroups of the backward pass, each of which leaves one row of partial sums: a function of the sizes alone, so the order
+// of the sums is the same on every call.
+int64_t bwd_parts(int64_t rows, int64_t cols)
+{
+    if (rows <= 0) return 0;
+    if (cols > AZ_NORM_MAX_COLS) return std::min<int64_t>(rows, 64);
+    const int64_t groups = cols <= 64 ? 16 : cols <= 1024 ? 4 : 1;
+    return std::min<int64_t>((rows + groups - 1) / groups, 1024);
+}
+
+struct BwdForm {
+    const NormBwd &a; hipStream_t st;
+    template <typename T, int TPR, int NV> void operator()() const
+    {
+        k_layer_norm_bwd<T, TPR, NV><<<(unsigned)bwd_parts(a.rows, a.cols), AZ_NORM_THREADS, 0, st>>>(a);
+    }
+};
+struct BwdType {
+    const NormBwd &a; void *dw, *db; hipStream_t st;
+    template <typename T> void operator()() const
+    {
+        const int64_t parts = bwd_parts(a.rows, a.cols);
+        if (parts > 0) {
+            if (a.cols > AZ_NORM_MAX_COLS) {
+                if (a.dx) k_layer_norm_bwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2 * 256), AZ_NORM_WIDE_THREADS, 0, st>>>(a);
+                if (a.part) k_layer_norm_cols_wide<T><<<dim3((unsigned)((a.cols + 1023) / 1024), (unsigned)parts), AZ_NORM_THREADS, 0, st>>>(a);
+            } else {
+                norm_form<T>(a.cols, BwdForm{a, st});
+            }
+        }
+        if (dw || db)
+            k_layer_norm_cols<T><<<dim3((unsigned)((a.cols + 63) / 64), 2), 1024, 0, st>>>(a.part, parts, a.cols, dw, db, a.affine_f32);
+    }
+};
+
+int norm_sizes(int64_t rows, int64_t cols, int32_t type, int32_t affine_type, double eps)
+{
+    if (bad_type(type) || bad_type(affine_type)) return az_fail(AZ_ERR_ARG, "layer norm: unknown element type");
+    if (affine_type != type && affine_type != AZ_TYPE_F32) return az_fail(AZ_ERR_ARG, "layer norm: weight and bias are float32 or of the input's type");
+    if (rows < 0 || cols < 1 || cols > ((int64_t)1 << 31) || rows > ((int64_t)1 << 40)) return az_fail(AZ_ERR_ARG, "layer norm: bad number of rows or columns");
+    if (!(eps >= 0.0)) return az_fail(AZ_ERR_ARG, "layer norm: eps must not be negative");
+    return AZ_OK;
+}
+
+}  // namespace
+
+extern "C" int az_layer_norm_fwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, double eps,
+                                     const void *x, int64_t x_stride, const void *weight, const void *bias, void *y, int64_t y_stride, float *mean, float *rstd)
+{
+    const int rc = norm_sizes(rows, cols, type, affine_type, eps);
+    if (rc) return rc;
+    if (rows == 0) return AZ_OK;
+    if (!x || !y) return az_fail(AZ_ERR_ARG, "layer norm: null array");
+    if (!mean != !rstd) return az_fail(AZ_ERR_ARG, "layer norm: mean and rstd go together");
+    if (x_stride < 0 || (y_stride < cols && rows > 1)) return az_fail(AZ_ERR_ARG, "layer norm: bad row stride");
+    DeviceScope scope(device);
+    if (scope.error != hipSuccess) return fail_hip("layer norm: device", scope.error);
+    const NormFwd a{x, weight, bias, y, mean, rstd, rows, cols, x_stride, y_stride, (float)eps, affine_type == AZ_TYPE_F32};
+    by_type(type, FwdType{a, static_cast<hipStream_t>(stream)});
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? AZ_OK : fail_hip("layer norm", e);
+}
+
+extern "C" int64_t az_layer_norm_bwd_workspace(int64_t rows, int64_t cols)
+{
+    return rows < 0 || cols < 1 ? 0 : 2 * bwd_parts(rows, cols) * cols;
+}
+
+extern "C" int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, const void *dy, int64_t dy_stride,
+                                     const void *x, int64_t x_stride, const void *weight, const float *mean, const float *rstd, void *dx, int64_t dx_stride,
+                                     void *dweight, void *dbias, float *workspace, int64_t workspace_floats)
+{
+    const int rc = norm_sizes(rows, cols, type, affine_type, 0.0);
+    if (rc) return rc;
+    if (rows > 0 && (!dy || !x || !mean || !rstd)) return az_fail(AZ_ERR_ARG, "layer norm backward: null array");
+    if (dy_stride < 0 || x_stride < 0 || (dx && dx_stride < cols && rows > 1)) return az_fail(AZ_ERR_ARG, "layer norm backward: bad row stride");
+    const bool sums = dweight || dbias;
+    const int64_t need = az_layer_norm_bwd_workspace(rows, cols);
+    if (sums && need > 0 && (!workspace || workspace_floats < need)) return az_fail(AZ_ERR_ARG, "layer norm backward: workspace smaller than az_layer_norm_bwd_workspace");
+    if (!dx && !sums) return AZ_OK;
+    DeviceScope scope(device);
+    if (scope.error != hipSuccess) return fail_hip("layer norm backward: device", scope.error);
+    const NormBwd a{dy, x, weight, mean, rstd, dx, sums ? workspace : nullptr, rows, cols, dy_stride, x_stride, dx_stride, affine_type == AZ_TYPE_F32};
+    by_type(type, BwdType{a, dweight, dbias, static_cast<hipStream_t>(stream)});
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? AZ_OK : fail_hip("layer norm backward", e);
+}
+
+namespace {
+
+struct Range {
+    uintptr_t first, end;
+    bool written;
+    bool operator<(const Range &o) const { return first < o.first; }
+};
+
+// Every element that a step writes belongs to one tensor only, and no gradient lies where something is written: workgroups
+// that share memory would race.  Gradients may share memory with each other.
+bool overlap(std::vector<Range> &r)
+{
+    std::sort(r.begin(), r.end());
+    uintptr_t read_end = 0, write_end = 0;   // of the ranges that start at or before the present one
+    for (const Range &x : r) {
+        if (x.first < write_end || (x.written && x.first < read_end)) return true;
+        uintptr_t &end = x.written ? write_end : read_end;
+        end = std::max(end, x.end);
+    }
+    return false;
+}
+
+struct AdamwType {
+    const AdamwTable &t; const AdamwScalars &k; unsigned blocks; bool eight; int turns; hipStream_t st;
+    template <typename T> void operator()() const
+    {
+        if (eight) {
+            if (turns == 1) k_adamw_8<T, 1><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+            else k_adamw_8<T, 2><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+        } else {
+            if (turns == 1) k_adamw_32<T, 1><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+            else k_adamw_32<T, 2><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+        }
+    }
+};
+
+int adamw_step(int32_t device, void *stream, int64_t tensors, void *const *params, const void *const *grads, void *const *m, void *const *v, float *const *m_scales,
+               float *const *v_scales, const int64_t *numels, int32_t type, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step)
+{
+    if (tensors < 0 || (tensors > 0 && (!params || !grads || !m || !v || !numels))) return az_fail(AZ_ERR_ARG, "adamw: null table");
+    if (bad_type(type)) return az_fail(AZ_ERR_ARG, "adamw: unknown element type");
+    if (!m_scales != !v_scales) return az_fail(AZ_ERR_ARG, "adamw: the scales of both states or of neither");
+    if (!(lr >= 0.0) || !(eps >= 0.0) || !(weight_decay >= 0.0)) return az_fail(AZ_ERR_ARG, "adamw: lr, eps and weight_decay must not be negative");
+    if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0)) return az_fail(AZ_ERR_ARG, "adamw: betas must lie in [0, 1)");
+    if (step < 1) return az_fail(AZ_ERR_ARG, "adamw: steps are counted from 1");
+    const bool eight = m_scales != nullptr;
+    const int64_t size = type == AZ_TYPE_F32 ? 4 : 2;
+    std::vector<Range> ranges;
+    ranges.reserve((size_t)tensors * (eight ? 6 : 4));
+    int64_t total = 0;
+    for (int64_t i = 0; i < tensors; i++) {
+        const int64_t n = numels[i];
+        if (n < 0 || n > ((int64_t)1 << 40)) return az_fail(AZ_ERR_ARG, "adamw: bad tensor size");
+        if (n == 0) continue;
+        if (!params[i] || !grads[i] || !m[i] || !v[i] || (eight && (!m_scales[i] || !v_scales[i]))) return az_fail(AZ_ERR_ARG, "adamw: null tensor");
+        const auto add = [&](const void *p, int64_t bytes, bool written = true) { ranges.push_back(Range{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written}); };
+        add(grads[i], n * size, false);
+        add(params[i], n * size);
+        add(m[i], eight ? n : n * 4);
+        add(v[i], eight ? n : n * 4);
+        if (eight) {
+            add(m_scales[i], (n + AZ_ADAMW_BLOCK - 1) / AZ_ADAMW_BLOCK * 4);
+            add(v_scales[i], (n + AZ_ADAMW_BLOCK - 1) / AZ_ADAMW_BLOCK * 4);
+        }
+        total += n;
+    }
+    if (total == 0) return AZ_OK;
+    if (overlap(ranges)) return az_fail(AZ_ERR_ARG, "adamw: two tensors share memory that the step writes");
+    DeviceScope scope(device);
+    if (scope.error != hipSuccess) return fail_hip("adamw: device", scope.error);
+    AdamwScalars k;
+    k.beta1 = beta1; k.beta2 = beta2; k.one_minus_beta1 = 1.0 - beta1; k.one_minus_beta2 = 1.0 - beta2;
+    k.decay = (float)(lr * weight_decay);
+    k.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+    k.inv_sqrt_c2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+    k.eps = (float)eps;
+    const int turns = total <= ((int64_t)1 << 20) ? 1 : 2;
+    const int64_t chunk = turns * 4 * AZ_ADAMW_THREADS;
+    AdamwTable t;
+    int held = 0;
+    uint64_t blocks = 0;
+    for (int64_t i = 0; i <= tensors; i++) {
+        const int64_t need = i < tensors ? (numels[i] + chunk - 1) / chunk : 0;
+        // a launch is full at 56 tensors, or when its workgroups would no longer fit the grid
+        if (held && (i == tensors || held == AZ_ADAMW_TENSORS || blocks + need > 0x40000000u)) {
+            for (int j = held; j < AZ_ADAMW_TENSORS; j++) t.last[j] = 0xffffffffu;
+            by_type(type, AdamwType{t, k, (unsigned)blocks, eight, turns, static_cast<hipStream_t>(stream)});
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return fail_hip("adamw", e);
+            held = 0;
+            blocks = 0;
+        }
+        if (i == tensors || need == 0) continue;
+        blocks += need;
+        t.param[held] = params[i]; t.grad[held] = grads[i]; t.m[held] = m[i]; t.v[held] = v[i];
+        t.m_scale[held] = eight ? m_scales[i] : nullptr; t.v_scale[held] = eight ? v_scales[i] : nullptr;
+        t.n[held] = numels[i];
+        t.last[held++] = (uint32_t)blocks;
+    }
+    return AZ_OK;
+}
+
+}  // namespace
+
+extern "C" int az_adamw_step_dev(int32_t device, void *stream, int64_t tensors, void *const *params, const void *const *grads, void *const *exp_avg,
+                                 void *const *exp_avg_sq, float *const *exp_avg_scale, float *const *exp_avg_sq_scale, const int64_t *numels, int32_t type,
+                                 double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step)
+{
+    try {
+        return adamw_step(device, stream, tensors, params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numels, type, lr, beta1, beta2, eps, weight_decay, step);
+    } catch (...) {   // (the list of ranges could not be allocated: nothing has been launched)
+        return az_fail(AZ_ERR_ARG, "adamw: out of host memory");
+    }
+}
+
+extern "C" int az_dequantize_state_dev(int32_t device, void *stream, const void *codes, const float *scales, int64_t n, int32_t is_signed, float *out)
+{
+    if (n < 0 || n > ((int64_t)1 << 40)) return az_fail(AZ_ERR_ARG, "dequantize: bad size");
+    if (n == 0) return AZ_OK;
+    if (!codes || !scales || !out) return az_fail(AZ_ERR_ARG, "dequantize: null array");
+    DeviceScope scope(device);
+    if (scope.error != hipSuccess) return fail_hip("dequantize: device", scope.error);
+    const int64_t per = AZ_ADAMW_THREADS * 4;
+    const unsigned blocks = (unsigned)std::min<int64_t>((n + per - 1) / per, 16 * 256);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const uint8_t *c = static_cast<const uint8_t *>(codes);
+    if (is_signed) k_dequantize_state<true><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(c, scales, n, out);
+    else k_dequantize_state<false><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(c, scales, n, out);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? AZ_OK : fail_hip("dequantize", e);
+}

@@ -163,7 +163,7 @@ az_engine *az_engine_create(const az_config *cfg);
  * az_engine_create (no handle needed).  No counterpart in the reference, which has no FFI. */
 void az_abi_sizes(int32_t out[3]);
 void az_engine_destroy(az_engine *h);
-const char *az_last_error(az_engine *h);       /* h may be NULL (creation errors) */
+const char *az_last_error(az_engine *h);       /* h may be NULL (creation errors, calls without a handle; per thread) */
 int az_engine_dims(az_engine *h, int32_t *n_slots, int32_t *cells, int32_t *actions);
 
 /* ---- game state (env/go.py, env/reversi.py, env/mnk.py GameState) ----- */
@@ -329,6 +329,43 @@ int az_tower_profile(az_engine *h, int32_t on);
  * the same either way, on=0 only serves comparisons. Applies where the tower's kernels take the row count from device
  * memory (256-channel bf16 tower, large batches) and never while az_tower_profile is on. */
 int az_tower_leaf_compaction(az_engine *h, int32_t on);
+
+/* ---- training operators ------------------------------------------------ */
+/* What the optimizer process (network/main.py:66-109, network/model.py:90-99) trains with, next to the libraries' convolutions
+ * and products.  No counterpart in the reference, which has batch norm and momentum SGD only.  These calls need no engine:
+ * `device` is the HIP device of the arrays and `stream` a stream of that device (NULL: its default stream), on which the work is
+ * queued - they return without waiting.  All arrays are device memory, element types are AZ_TYPE_*.  The calling thread's
+ * current device is left as it was.  Any number of threads may call at once.  az_last_error(NULL) says why a call failed. */
+#define AZ_TYPE_F32 0
+#define AZ_TYPE_BF16 1
+#define AZ_TYPE_F16 2
+/* Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias for `rows` rows of `cols` elements; row i of x
+ * starts at element i * x_stride (0: the same row throughout).  weight / bias may be NULL (1 / 0) and are of affine_type, float32 or
+ * x's type.  mean / rstd (float32, [rows]): what the backward pass needs, or both NULL. */
+int az_layer_norm_fwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, double eps,
+                          const void *x, int64_t x_stride, const void *weight, const void *bias, void *y, int64_t y_stride,
+                          float *mean, float *rstd);
+/* Its gradient: dx (of x's type), dweight and dbias (of affine_type, sums over the rows, the same bits on every call); each may
+ * be NULL if not wanted.  workspace: az_layer_norm_bwd_workspace(rows, cols) floats, needed for dweight / dbias; it may be reused
+ * as soon as the stream has passed the call. */
+int64_t az_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
+int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, const void *dy,
+                          int64_t dy_stride, const void *x, int64_t x_stride, const void *weight, const float *mean, const float *rstd,
+                          void *dx, int64_t dx_stride, void *dweight, void *dbias, float *workspace, int64_t workspace_floats);
+/* One AdamW step over `tensors` tensors (host tables of device pointers, read before the call returns):
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   w = w - lr weight_decay w - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+ * params and grads are of `type`, numels[i] elements each in the same order.  exp_avg_scale / exp_avg_sq_scale NULL: m and v
+ * are float32.  Otherwise m is int8 and v uint8 codes in blocks of AZ_STATE_BLOCK elements with one float32 scale s each:
+ *   m = s sgn(c) (c / 127)^2,  v = s (c / 255)^4.
+ * Nothing that is written may overlap (AZ_ERR_ARG).  The scalars are fixed at the call: a captured graph would replay the same
+ * step number, so capture is the caller's to avoid. */
+#define AZ_STATE_BLOCK 256
+int az_adamw_step_dev(int32_t device, void *stream, int64_t tensors, void *const *params, const void *const *grads, void *const *exp_avg,
+                      void *const *exp_avg_sq, float *const *exp_avg_scale, float *const *exp_avg_sq_scale, const int64_t *numels,
+                      int32_t type, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step);
+/* The values that n codes of such a state stand for (is_signed 1: m, 0: v). */
+int az_dequantize_state_dev(int32_t device, void *stream, const void *codes, const float *scales, int64_t n, int32_t is_signed, float *out);
 
 /* ---- measurement ------------------------------------------------------ */
 int az_counters_get(az_engine *h, az_counters *out);
