@@ -2,6 +2,7 @@
 `eval(state) -> ([(action, prob)] in index order, value)`, `load(path)`, `save(path)`, `.rwlock`,
 context manager.  The network runs in the HIP tower of an engine owned by this object; there is
 no listener process and no queue - batching happens inside the engine across game slots."""
+import copy
 import threading
 
 import numpy as np
@@ -44,22 +45,31 @@ class RWLock:
 
 
 class NNEvaluator:
-    def __init__(self, game_config, num_blocks=19, channels=256, dtype="bf16", max_batch_size=32, seed=0, net=None, device=0):
+    """`norm="layer"` (or a `net` with layer norm) cannot be folded into the tower: PyTorch evaluates such a network on the
+    same GPU, in float32, whatever `dtype` says, and searches treat the evaluator as they treat any other that is not a tower."""
+
+    def __init__(self, game_config, num_blocks=19, channels=256, dtype="bf16", max_batch_size=32, seed=0, net=None, device=0, norm="batch"):
         self.game_config = game_config
         self.num_blocks, self.channels, self.dtype = num_blocks, channels, dtype
         kw = game_config_to_engine_kwargs(game_config)
         self._H, self._W, self._O = kw["board_height"], kw["board_width"], game_config['flat_move_output']
-        self.net = net if net is not None else random_net(self._H, self._W, self._O, num_blocks, channels, seed=seed)
+        self.net = net if net is not None else random_net(self._H, self._W, self._O, num_blocks, channels, seed=seed, norm=norm)
         self.rwlock = RWLock()
-        self._eng = Engine(n_slots=max_batch_size, num_blocks=num_blocks, channels=channels, tower_dtype=dtype, device=device, **kw)
+        if self.net.norm == "batch":
+            self._eng = Engine(n_slots=max_batch_size, num_blocks=num_blocks, channels=channels, tower_dtype=dtype, device=device, **kw)
+        else:
+            self._eng, self._device = None, torch.device("cuda", device)
         self._conv = StateTensorConverter(game_config)
         self._t2a = TensorActionConverter(game_config)
         self.version = 0
         self._refold()
 
     def _refold(self):
-        self._tower_blob = fold_to_blob(self.net)
-        self._eng.tower_load(self._tower_blob)
+        if self._eng is not None:
+            self._tower_blob = fold_to_blob(self.net)
+            self._eng.tower_load(self._tower_blob)
+        else:   # a copy, as the tower's: training self.net further changes nothing here until the next load / set_weights
+            self._net = copy.deepcopy(self.net).to(self._device).eval()
         self.version += 1
 
     def __enter__(self):
@@ -70,12 +80,16 @@ class NNEvaluator:
 
     def eval(self, state):
         planes = self._conv.state_to_tensor(state)
-        p, v = self._eng.tower_forward(planes)
+        p, v = self.eval_batch(planes)
         return self._t2a.tensor_to_action(p[0]), v[0]
 
     def eval_batch(self, planes):
         """planes int8 (B,17,H,W) -> (priors float32 (B,O), values float32 (B,)): Network.response."""
-        return self._eng.tower_forward(planes)
+        if self._eng is not None:
+            return self._eng.tower_forward(planes)
+        with torch.no_grad():
+            p, v, _ = self._net(torch.as_tensor(np.asarray(planes), dtype=torch.float32, device=self._device))
+        return p.cpu().numpy(), v.cpu().numpy()
 
     def load(self, filename):
         self.rwlock.w_acquire()

@@ -131,6 +131,13 @@ def grow_pool_when_used(eng, share=0.8):
     return False
 
 
+def tower_kwargs(nn_eval):
+    """Engine arguments for an evaluator's network: its tower, or none for a network that only PyTorch evaluates."""
+    if not hasattr(nn_eval, "_tower_blob"):
+        return {}
+    return dict(num_blocks=nn_eval.num_blocks, channels=nn_eval.channels, tower_dtype=nn_eval.dtype)
+
+
 class BatchedSelfplay:
     """`n_games` concurrent self-play games on one GPU; the role of Selfplay.run +
     selfplay_wrapper (train/parallel/selfplay.py:71-108) without a process per game.
@@ -150,6 +157,9 @@ class BatchedSelfplay:
     for all of them - finished slots are not re-armed until every game in flight has ended, then the weights are
     loaded and all slots start again, so no game ever sees two networks.
 
+    A network that the tower cannot hold (layer norm) is evaluated through nn_eval.eval_batch, once per round for all
+    games together, with the planes and priors passing through host memory.
+
     rng_streams: optional list of (transform ids, gamma draws, uniforms), one per slot - the engine then replays these
     draws instead of using its own generator (parity tests)."""
 
@@ -163,15 +173,15 @@ class BatchedSelfplay:
         kw = game_config_to_engine_kwargs(game_config)
         self.eng = Engine(n_slots=n_games, max_playout=ext_config['player']['max_playout'],
                           dirichlet_before=ext_config['dirichlet_before'], max_turn=ext_config['max_turn'],
-                          record_trajectories=True, seed=seed, num_blocks=nn_eval.num_blocks, channels=nn_eval.channels,
-                          tower_dtype=nn_eval.dtype, device=device, tree_full_policy=1, rng_replay=rng_streams is not None,
-                          tree_pool_edges=tree_pool_edges, **kw)
+                          record_trajectories=True, seed=seed, device=device, tree_full_policy=1, rng_replay=rng_streams is not None,
+                          tree_pool_edges=tree_pool_edges, **tower_kwargs(nn_eval), **kw)
         if rng_streams is not None:
             if len(rng_streams) != n_games:
                 raise ValueError("one (tids, etas, unis) triple per slot")
             for s, st in enumerate(rng_streams):
                 self.eng.rng_inject(s, *st)
         self._nn_eval = nn_eval
+        self._tower = hasattr(nn_eval, "_tower_blob")
         self._version = None
         self._replay = Engine(n_slots=self.REPLAY_SLOTS, device=device, **kw)
         self.n_games = n_games
@@ -184,7 +194,8 @@ class BatchedSelfplay:
 
     def _sync_weights(self):
         if self._version != self._nn_eval.version:
-            self.eng.tower_load(self._nn_eval._tower_blob)
+            if self._tower:
+                self.eng.tower_load(self._nn_eval._tower_blob)
             self._version = self._nn_eval.version
 
     def _convert(self, popped):
@@ -192,6 +203,15 @@ class BatchedSelfplay:
         for i in range(0, len(popped), self.REPLAY_SLOTS):
             out += history_arrays_batch(self._replay, popped[i:i + self.REPLAY_SLOTS])
         return out
+
+    def _rounds(self, n):
+        if self._tower:
+            self.eng.selfplay_run(n)    # the C call releases the GIL: the worker converts meanwhile
+            return
+        for _ in range(n):
+            if self.eng.selfplay_select() == 0:
+                break
+            self.eng.selfplay_finish(*self._nn_eval.eval_batch(self.eng.leaf_batch()[0]))
 
     def _watch_pool(self):
         grow_pool_when_used(self.eng, self.POOL_GROW_AT)
@@ -217,7 +237,7 @@ class BatchedSelfplay:
         pending = []
         with ThreadPoolExecutor(max_workers=1) as pool:   # one worker: conversions stay in finishing order
             while len(slots) < num_games:
-                self.eng.selfplay_run(rounds_per_poll)    # the C call releases the GIL: the worker converts meanwhile
+                self._rounds(rounds_per_poll)
                 plies, done = self.eng.selfplay_status()
                 self._watch_pool()
                 fin = np.flatnonzero((done != 0) & ~self._empty)
@@ -265,6 +285,8 @@ class BatchedMatch:
     `n_parallel` (default: every game at once) replaces num_worker as the concurrency limit."""
 
     def __init__(self, nn_eval_chal, nn_eval_best, game_config, ext_config, n_parallel=None, seed=0, device=0):
+        if not (hasattr(nn_eval_chal, "_tower_blob") and hasattr(nn_eval_best, "_tower_blob")):
+            raise ValueError("BatchedMatch plays networks that the tower holds (batch norm); Game plays any evaluator")
         self.nn_eval_chal, self.nn_eval_best = nn_eval_chal, nn_eval_best
         self.game_config, self.ext_config = game_config, ext_config
         self.num_games = ext_config['num_games']

@@ -6,6 +6,10 @@ policy head 1x1 conv->2, BN, ReLU, NCHW flatten, FC->O, softmax; value head 1x1 
 FC->256, ReLU, FC->1, tanh.  TF's default initialiser (glorot uniform) and fresh BN statistics
 (mean 0, var 1, beta 0) are used for random initialisation.
 
+`norm="layer"` puts a layer norm in the place of every batch norm: over the channels of each point in the trunk, over
+the flattened planes in the two heads.  Such a network has no moving statistics, so it trains and plays with the same
+function at any batch size; it cannot be folded into the blob (its scale depends on the position), so PyTorch evaluates it.
+
 Blob layout (float32, BN already folded; tap = (dh+1)*3 + (dw+1) over the (H, W) axes):
     stem_w[C][9][17] stem_b[C]
     per block: w1[C][9][C] b1[C] w2[C][9][C] b2[C]
@@ -19,6 +23,8 @@ import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .layer_norm import LayerNorm
 
 BN_EPS = 1e-3  # tf.contrib.layers.batch_norm default epsilon
 
@@ -45,6 +51,20 @@ class CenterBN(nn.Module):
         return (x - mean[None, :, None, None]) / torch.sqrt(var[None, :, None, None] + BN_EPS) + self.beta[None, :, None, None]
 
 
+class PointNorm(LayerNorm):
+    """Layer norm over the channels of every point of (B, C, H, W), which are neighbours in memory (channels last)."""
+
+    def forward(self, x):
+        return super().forward(x.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
+
+
+class PlaneNorm(LayerNorm):
+    """Layer norm over all points of all planes of (B, C, H, W)."""
+
+    def forward(self, x):
+        return super().forward(x.flatten(1)).view(x.shape)
+
+
 def _glorot_conv(conv):
     co, ci, kh, kw = conv.weight.shape
     limit = math.sqrt(6.0 / (ci * kh * kw + co * kh * kw))
@@ -58,21 +78,27 @@ def _glorot_linear(lin):
 
 
 class AZNet(nn.Module):
-    def __init__(self, board_height, board_width, flat_move_output, num_blocks, channels=256, planes=17):
+    def __init__(self, board_height, board_width, flat_move_output, num_blocks, channels=256, planes=17, norm="batch"):
         super().__init__()
+        if norm not in ("batch", "layer"):
+            raise ValueError("norm must be 'batch' or 'layer', not %r" % (norm,))
+        self.norm = norm
+        points = board_height * board_width
+        trunk = CenterBN if norm == "batch" else PointNorm
+        head = CenterBN if norm == "batch" else (lambda c: PlaneNorm(c * points))
         self.H, self.W, self.O, self.NB, self.C, self.F = board_height, board_width, flat_move_output, num_blocks, channels, planes
         C = channels
         self.stem = nn.Conv2d(planes, C, 3, padding=1, bias=False)
-        self.stem_bn = CenterBN(C)
+        self.stem_bn = trunk(C)
         self.conv1 = nn.ModuleList([nn.Conv2d(C, C, 3, padding=1, bias=False) for _ in range(num_blocks)])
-        self.bn1 = nn.ModuleList([CenterBN(C) for _ in range(num_blocks)])
+        self.bn1 = nn.ModuleList([trunk(C) for _ in range(num_blocks)])
         self.conv2 = nn.ModuleList([nn.Conv2d(C, C, 3, padding=1, bias=False) for _ in range(num_blocks)])
-        self.bn2 = nn.ModuleList([CenterBN(C) for _ in range(num_blocks)])
+        self.bn2 = nn.ModuleList([trunk(C) for _ in range(num_blocks)])
         self.p_conv = nn.Conv2d(C, 2, 1, bias=False)
-        self.p_bn = CenterBN(2)
+        self.p_bn = head(2)
         self.p_fc = nn.Linear(2 * board_height * board_width, flat_move_output)
         self.v_conv = nn.Conv2d(C, 1, 1, bias=False)
-        self.v_bn = CenterBN(1)
+        self.v_bn = head(1)
         self.v_fc1 = nn.Linear(board_height * board_width, 256)
         self.v_fc2 = nn.Linear(256, 1)
         for m in self.modules():
@@ -80,8 +106,12 @@ class AZNet(nn.Module):
                 _glorot_conv(m)
             elif isinstance(m, nn.Linear):
                 _glorot_linear(m)
+        if norm == "layer":
+            self.to(memory_format=torch.channels_last)
 
     def forward(self, x):
+        if self.norm == "layer":
+            x = x.contiguous(memory_format=torch.channels_last)
         r = F.relu(self.stem_bn(self.stem(x)))
         for i in range(self.NB):
             r1 = F.relu(self.bn1[i](self.conv1[i](r)))
@@ -106,6 +136,8 @@ def _fold(conv, bn):
 
 def fold_to_blob(net):
     """BN-folded float32 weight blob in the layout az_tower_load_weights expects."""
+    if net.norm != "batch":
+        raise ValueError("a network with layer norm cannot be folded into the tower's weights")
     parts = []
 
     def put(t):
@@ -125,12 +157,12 @@ def fold_to_blob(net):
     return np.concatenate(parts).astype(np.float32)
 
 
-def random_net(board_height, board_width, flat_move_output, num_blocks, channels=256, seed=0, perturb_bn=False):
+def random_net(board_height, board_width, flat_move_output, num_blocks, channels=256, seed=0, perturb_bn=False, norm="batch"):
     """Seeded glorot-uniform network; perturb_bn randomises BN statistics so folding is exercised."""
     g = torch.Generator().manual_seed(seed)
     state = torch.random.get_rng_state()
     torch.manual_seed(seed)
-    net = AZNet(board_height, board_width, flat_move_output, num_blocks, channels)
+    net = AZNet(board_height, board_width, flat_move_output, num_blocks, channels, norm=norm)
     if perturb_bn:
         for m in net.modules():
             if isinstance(m, CenterBN):

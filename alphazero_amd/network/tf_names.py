@@ -26,6 +26,8 @@ def _bn_items(prefix, bn):
 
 def _entries(net):
     """[(tf_name, tensor, kind)] in graph construction order; kind: conv | linear_w | vec."""
+    if net.norm != "batch":
+        raise ValueError("the reference's graph has batch norm: a network with layer norm has no names in it")
     out = [("model/W0", net.stem.weight, "conv")]
     out += [(n, t, "vec") for n, t in _bn_items("model/bn", net.stem_bn)]
     for i in range(net.NB):

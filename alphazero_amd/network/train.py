@@ -9,6 +9,10 @@ w -= lr*accum, tf.train.MomentumOptimizer) with the piecewise-constant schedule 
 (tf.train.piecewise_constant(step, boundaries[1:], values): values[i] holds while step <= boundary i).
 Batch norm in training mode uses batch statistics and updates the moving averages with `batch_decay`.
 
+Beyond the reference: `optimizer: adamw` or `adamw8` in the training config takes AdamW (network/adamw.py) in the place of the
+momentum SGD, with its state in 32 or 8 bits; the keys betas, eps and weight_decay (0.9 / 0.999, 1e-8, 1e-2) belong to it, and
+`l2` stays what it is, a term of the loss.  `norm: layer` takes layer norm in the place of batch norm (network/model.py).
+
 Parity note: TensorFlow is absent and the reference has no test for this path, so the arithmetic is
 checked against an independent NumPy restatement of the formulas above, not against TF (unpinned).
 """
@@ -19,6 +23,7 @@ import torch
 import torch.nn.functional as F
 import yaml
 
+from .adamw import AdamW
 from .model import AZNet, CenterBN
 
 _DEFAULT_TRAIN_CONFIG = {
@@ -44,6 +49,17 @@ def az_loss(logits, v_hat, p, z, params, l2, mse_scaling):
     return p_loss + v_loss * mse_scaling + r_loss
 
 
+def make_optimizer(params, cfg):
+    """The optimizer that a training config names: momentum SGD (the reference's, the default), adamw or adamw8."""
+    kind, lr = cfg.get("optimizer", "momentum"), piecewise_lr(0, cfg["learning_rate"])
+    if kind == "momentum":
+        return torch.optim.SGD(params, lr=lr, momentum=float(cfg["momentum"]), dampening=0.0, nesterov=False)
+    if kind not in ("adamw", "adamw8"):
+        raise ValueError("optimizer must be 'momentum', 'adamw' or 'adamw8', not %r" % (kind,))
+    return AdamW(params, lr=lr, betas=tuple(float(b) for b in cfg.get("betas", (0.9, 0.999))), eps=float(cfg.get("eps", 1e-8)),
+                 weight_decay=float(cfg.get("weight_decay", 1e-2)), state_bits=8 if kind == "adamw8" else 32)
+
+
 class Network:
     def __init__(self, game_config, num_gpu=1, train_config=None, load_pretrained=False, device=None, channels=256):
         if train_config is None:
@@ -57,13 +73,12 @@ class Network:
         self._game_config = game_config
         self.device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
         self.net = AZNet(game_config["board_height"], game_config["board_width"], game_config["flat_move_output"],
-                         cfg["num_blocks"], channels).to(self.device)
+                         cfg["num_blocks"], channels, norm=cfg.get("norm", "batch")).to(self.device)
         for m in self.net.modules():
             if isinstance(m, CenterBN):
                 m.decay = float(cfg["batch_decay"])
         self.global_step = 0
-        self.opt = torch.optim.SGD(self.net.parameters(), lr=piecewise_lr(0, cfg["learning_rate"]),
-                                   momentum=float(cfg["momentum"]), dampening=0.0, nesterov=False)
+        self.opt = make_optimizer(self.net.parameters(), cfg)
         if load_pretrained:
             # network/main.py:92-95 restores tf.train.latest_checkpoint(save_dir): the newest '<prefix>-<step>' of save()
             path = latest_checkpoint(cfg["save_dir"])
@@ -118,11 +133,14 @@ class Network:
 
     def load(self, filename):
         """A file of save(), or a bare state dict as NNEvaluator.save writes it (weights only: step and optimizer
-        state are then left as they are)."""
+        state are then left as they are).  A file of another optimizer is refused (adamw and adamw8 take each other's)."""
         ck = torch.load(filename, weights_only=True, map_location=self.device)
         if "model" not in ck:
             self.net.load_state_dict(ck)
             return
+        of_adamw = "betas" in ck["opt"]["param_groups"][0]
+        if of_adamw != isinstance(self.opt, AdamW):
+            raise ValueError("%r holds the state of %s" % (filename, "an AdamW optimizer" if of_adamw else "a momentum optimizer"))
         self.net.load_state_dict(ck["model"])
         self.opt.load_state_dict(ck["opt"])
         self.global_step = int(ck["global_step"])
