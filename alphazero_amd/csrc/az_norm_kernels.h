@@ -8,14 +8,17 @@
 // registers, in a second pass over those registers: a sum of squares would lose everything in rows whose mean is large
 // against their spread.
 //
-// A row belongs to TPR threads (16: a quarter of a wave, 64: a wave, 256: a workgroup), each of which holds NV groups of four
-// neighbouring elements in registers, so a row is read from memory once.  Workgroups walk the rows with a stride, so that
-// weights and biases are loaded once per thread and not once per row.
+// A row belongs to TPR threads (16 or 32: part of a wave, 64: a wave, more: a workgroup), each of which holds NV packs of 16
+// bytes of it in registers, so a row is read from memory once; the up to 3 or 7 elements past the last whole pack are held one
+// to a thread.  Workgroups walk the rows with a stride: weights and biases
+// are loaded once per thread and not once per row, and the next row is asked for before the present one is worked on.
 #pragma once
 #include "az_vec.h"
 
-#define AZ_NORM_THREADS 256
 #define AZ_NORM_WIDE_THREADS 1024
+#define AZ_NORM_COLS_WIDE_THREADS 256
+
+constexpr int norm_threads(int tpr) { return tpr > 256 ? tpr : 256; }
 
 // weights and biases: float32 or the element type; absent ones are 1 and 0
 template <typename T> __device__ __forceinline__ float4 load_affine(const void *p, bool f32, int64_t i, int64_t n, float absent)
@@ -24,25 +27,60 @@ template <typename T> __device__ __forceinline__ float4 load_affine(const void *
     return f32 ? load4(static_cast<const float *>(p), i, n) : load4(static_cast<const T *>(p), i, n);
 }
 
-__device__ __forceinline__ float sum4(float4 f) { return (f.x + f.y) + (f.z + f.w); }
-
-// Sums of TPR threads' values in each of them.  With a whole workgroup per row the four waves meet in LDS; `slot` alternates
-// between two pairs of cells, so that one barrier per sum is enough: a cell is written again only after the other sum's barrier.
-template <int TPR, int N> __device__ __forceinline__ void group_sum(float (&v)[N], float (*cell)[AZ_NORM_THREADS / 64][2], int slot)
+template <typename T> __device__ __forceinline__ void load_affine_pack(const void *p, bool f32, int i, bool in, float absent, float (&out)[Pack<T>::N])
 {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = TPR == 16 ? row16_sum(v[i]) : wave_sum(v[i]);
-    if constexpr (TPR == AZ_NORM_THREADS) {
+    for (int e = 0; e < Pack<T>::N; e += 4) {
+        const float4 f = load_affine<T>(in ? p : nullptr, f32, i + e, i + e + 4, absent);
+        out[e] = f.x; out[e + 1] = f.y; out[e + 2] = f.z; out[e + 3] = f.w;
+    }
+}
+
+template <typename T> __device__ __forceinline__ float load_affine_one(const void *p, bool f32, int i, bool in, float absent)
+{
+    if (!p || !in) return absent;
+    return f32 ? static_cast<const float *>(p)[i] : (float)static_cast<const T *>(p)[i];
+}
+
+__device__ __forceinline__ float sum4(float4 f) { return (f.x + f.y) + (f.z + f.w); }
+
+// Sums of TPR threads' values in each of them.  With a whole workgroup per row the waves meet in LDS; `slot` alternates
+// between two sets of cells, so that one barrier per sum is enough: a cell is written again only after the other sum's barrier.
+template <int TPR, int N> __device__ __forceinline__ void group_sum(float (&v)[N], float (*cell)[N][16], int slot)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = TPR == 16 ? row16_sum(v[i]) : TPR == 32 ? half_sum(v[i]) : wave_sum(v[i]);
+    if constexpr (TPR > 64) {
+        constexpr int WAVES = TPR / 64;
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int i = 0; i < N; i++) cell[slot][wave][i] = v[i];
+            for (int i = 0; i < N; i++) cell[slot][i][wave] = v[i];
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = (cell[slot][0][i] + cell[slot][1][i]) + (cell[slot][2][i] + cell[slot][3][i]);
+        for (int i = 0; i < N; i++) {
+            float s[WAVES];
+#pragma unroll
+            for (int j = 0; j < WAVES; j++) s[j] = cell[slot][i][j];
+#pragma unroll
+            for (int d = WAVES / 2; d > 0; d >>= 1)
+#pragma unroll
+                for (int j = 0; j < d; j++) s[j] += s[j + d];
+            v[i] = s[0];
+        }
     }
 }
+
+// s / n, exact where the quotient is: rows of one value come out with exactly that mean
+__device__ __forceinline__ float mean_of(float s, float n, float inv)
+{
+    const float q = s * inv;
+    return fmaf(fmaf(-q, n, s), inv, q);
+}
+
+// 1 / sqrt(t) to one step of float32; the instruction takes no subnormal numbers
+__device__ __forceinline__ float inv_sqrt(float t) { return t < 0x1p-126f ? 1.0f / sqrtf(t) : __builtin_amdgcn_rsqf(t); }
 
 struct NormFwd {
     const void *x, *w, *b;
@@ -50,54 +88,83 @@ struct NormFwd {
     float *mean, *rstd;      // may be null
     int64_t rows, cols, x_stride, y_stride;
     float eps;
-    bool affine_f32;
+    bool affine_f32, stream; // stream: y is larger than the L2 caches
 };
 
-template <typename T, int TPR, int NV> __global__ __launch_bounds__(AZ_NORM_THREADS) void k_layer_norm_fwd(NormFwd a)
+template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads(TPR)) void k_layer_norm_fwd(NormFwd a)
 {
-    __shared__ float cell[2][AZ_NORM_THREADS / 64][2];
-    constexpr int GROUPS = AZ_NORM_THREADS / TPR;
-    const int t = threadIdx.x % TPR;
-    const float inv = 1.0f / (float)a.cols;
-    float4 w[NV], b[NV];
+    constexpr int N = Pack<T>::N, GROUPS = norm_threads(TPR) / TPR;
+    __shared__ float cell[2][1][16];
+    const int t = threadIdx.x % TPR, cols = (int)a.cols, packs = cols / N, last = packs * N + t;
+    const bool full = packs == TPR * NV, tail = last < cols;
+    const float n = (float)cols, inv = 1.0f / n;
+    float w[NV][N], b[NV][N];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const int64_t c = (int64_t)(k * TPR + t) * 4;
-        w[k] = load_affine<T>(a.w, a.affine_f32, c, a.cols, 1.0f);
-        b[k] = load_affine<T>(a.b, a.affine_f32, c, a.cols, 0.0f);
+        load_affine_pack<T>(a.w, a.affine_f32, (k * TPR + t) * N, k * TPR + t < packs, 1.0f, w[k]);
+        load_affine_pack<T>(a.b, a.affine_f32, (k * TPR + t) * N, k * TPR + t < packs, 0.0f, b[k]);
     }
-    // the number of turns is the same for every thread of a workgroup: lanes whose row is past the end sum zeros
-    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += (int64_t)gridDim.x * GROUPS) {
-        const int64_t row = first + threadIdx.x / TPR;
-        const bool in = row < a.rows;
-        const int64_t cols = in ? a.cols : 0;
-        const T *x = static_cast<const T *>(a.x) + (in ? row : 0) * a.x_stride;
-        float4 v[NV];
-        float s[1] = {0.f};
-#pragma unroll
-        for (int k = 0; k < NV; k++) v[k] = load4(x, (int64_t)(k * TPR + t) * 4, cols);
-#pragma unroll
-        for (int k = 0; k < NV; k++) s[0] += sum4(v[k]);
-        group_sum<TPR>(s, cell, 0);
-        const float mean = s[0] / (float)a.cols;   // (a division: rows of one value come out with exactly that mean)
-        float q[1] = {0.f};
+    const float w1 = load_affine_one<T>(a.w, a.affine_f32, last, tail, 1.0f), b1 = load_affine_one<T>(a.b, a.affine_f32, last, tail, 0.0f);
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
+    int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
+    typename Pack<T>::type next[NV];
+    T next1;
+    // a row past the end reads as zeros
+    const auto ask = [&](int64_t i) {
+        const T *x = static_cast<const T *>(a.x) + i * a.x_stride;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int64_t c = (int64_t)(k * TPR + t) * 4;
-            v[k].x = c < cols ? v[k].x - mean : 0.f;
-            v[k].y = c + 1 < cols ? v[k].y - mean : 0.f;
-            v[k].z = c + 2 < cols ? v[k].z - mean : 0.f;
-            v[k].w = c + 3 < cols ? v[k].w - mean : 0.f;
-            q[0] += (v[k].x * v[k].x + v[k].y * v[k].y) + (v[k].z * v[k].z + v[k].w * v[k].w);
+            next[k] = {};
+            if (i < a.rows && k * TPR + t < packs) next[k] = load_pack<false>(x + (k * TPR + t) * N);
         }
-        group_sum<TPR>(q, cell, 1);
-        const float r = 1.0f / sqrtf(q[0] * inv + a.eps);
-        T *y = static_cast<T *>(a.y) + (in ? row : 0) * a.y_stride;
+        next1 = T(0);
+        if (i < a.rows && tail) next1 = x[last];
+    };
+    ask(row);
+    // the number of turns is the same for every thread of a workgroup
+    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += step, row += step) {
+        float v[NV][N], v1 = (float)next1, s[1] = {v1}, q[1];
 #pragma unroll
         for (int k = 0; k < NV; k++)
-            store4(y, (int64_t)(k * TPR + t) * 4, cols,
-                   make_float4(v[k].x * r * w[k].x + b[k].x, v[k].y * r * w[k].y + b[k].y, v[k].z * r * w[k].z + b[k].z, v[k].w * r * w[k].w + b[k].w));
-        if (a.mean && in && t == 0) { a.mean[row] = mean; a.rstd[row] = r; }
+#pragma unroll
+            for (int e = 0; e < N; e++) v[k][e] = (float)next[k][e];
+        if (first + step < a.rows) ask(row + step);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < N; e += 4) s[0] += (v[k][e] + v[k][e + 1]) + (v[k][e + 2] + v[k][e + 3]);
+        group_sum<TPR>(s, cell, 0);
+        const float mean = mean_of(s[0], n, inv);
+        v1 = tail ? v1 - mean : 0.f;
+        q[0] = v1 * v1;
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[k][e] -= mean;
+        if (!full) {
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int e = 0; e < N; e++) v[k][e] = k * TPR + t < packs ? v[k][e] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < N; e += 4)
+                q[0] += (v[k][e] * v[k][e] + v[k][e + 1] * v[k][e + 1]) + (v[k][e + 2] * v[k][e + 2] + v[k][e + 3] * v[k][e + 3]);
+        group_sum<TPR>(q, cell, 1);
+        const float r = inv_sqrt(q[0] * inv + a.eps);
+        if (row < a.rows) {
+            T *y = static_cast<T *>(a.y) + row * a.y_stride;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+#pragma unroll
+                for (int e = 0; e < N; e++) v[k][e] = v[k][e] * r * w[k][e] + b[k][e];
+                if (k * TPR + t < packs) store_pack(y + (k * TPR + t) * N, v[k], a.stream);
+            }
+            if (tail) y[last] = (T)(v1 * r * w1 + b1);
+            if (a.mean && t == 0) { a.mean[row] = mean; a.rstd[row] = r; }
+        }
     }
 }
 
@@ -125,7 +192,7 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
         T *y = static_cast<T *>(a.y) + row * a.y_stride;
         float s = 0.f, q = 0.f;
         for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) s += sum4(load4(x, c, a.cols));
-        const float mean = block_sum(s, cell) / (float)a.cols;
+        const float mean = mean_of(block_sum(s, cell), (float)a.cols, inv);
         for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) {
             const float4 v = load4(x, c, a.cols);
             const float d0 = v.x - mean, d1 = v.y - mean, d2 = v.z - mean, d3 = v.w - mean;
@@ -134,7 +201,7 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
             if (c + 2 < a.cols) q += d2 * d2;
             if (c + 3 < a.cols) q += d3 * d3;
         }
-        const float r = 1.0f / sqrtf(block_sum(q, cell) * inv + a.eps);
+        const float r = inv_sqrt(block_sum(q, cell) * inv + a.eps);
         for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) {
             const float4 v = load4(x, c, a.cols), w = load_affine<T>(a.w, a.affine_f32, c, a.cols, 1.0f);
             const float4 b = load_affine<T>(a.b, a.affine_f32, c, a.cols, 0.0f);
@@ -150,61 +217,88 @@ struct NormBwd {
     void *dx;                // null: not wanted
     float *part;             // [2][parts][cols] sums of the workgroups' rows: dw, then db; null: not wanted
     int64_t rows, cols, dy_stride, x_stride, dx_stride;
-    bool affine_f32;
+    bool affine_f32, stream; // stream: dx is larger than the L2 caches
 };
 
 // dx of the rows, and for every workgroup the sums of dy * h and dy over its rows in the order in which it meets them: no
 // atomics, so the same call gives the same bits.  The threads of a workgroup that hold the same columns of different rows
 // add up through LDS at the end.
-template <typename T, int TPR, int NV> __global__ __launch_bounds__(AZ_NORM_THREADS) void k_layer_norm_bwd(NormBwd a)
+// Elements past a row's end need no masks: their dy reads as 0, so they add nothing to any sum, and they are not stored.
+// STREAM: x and dy, which this pass is the last to read, go past the L2 caches.
+template <typename T, int TPR, int NV, bool STREAM> __global__ __launch_bounds__(norm_threads(TPR)) void k_layer_norm_bwd(NormBwd a)
 {
-    constexpr int GROUPS = AZ_NORM_THREADS / TPR, WIDTH = TPR * NV * 4;
-    __shared__ float cell[2][AZ_NORM_THREADS / 64][2];
-    __shared__ float4 gather[GROUPS > 1 ? GROUPS * WIDTH / 4 : 1];
-    const int t = threadIdx.x % TPR;
-    const float inv = 1.0f / (float)a.cols;
-    float4 w[NV], dw[NV], db[NV];
+    constexpr int N = Pack<T>::N, THREADS = norm_threads(TPR), GROUPS = THREADS / TPR, WIDTH = (TPR * NV + 1) * N;
+    __shared__ float cell[2][2][16];
+    __shared__ float gather[GROUPS > 1 ? GROUPS * WIDTH : 1];
+    const int t = threadIdx.x % TPR, cols = (int)a.cols, packs = cols / N, last = packs * N + t;
+    const bool tail = last < cols;
+    const float inv = 1.0f / (float)cols;
+    float w[NV][N], dw[NV][N], db[NV][N], dw1 = 0.f, db1 = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        w[k] = load_affine<T>(a.w, a.affine_f32, (int64_t)(k * TPR + t) * 4, a.cols, 1.0f);
-        dw[k] = db[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        load_affine_pack<T>(a.w, a.affine_f32, (k * TPR + t) * N, k * TPR + t < packs, 1.0f, w[k]);
+#pragma unroll
+        for (int e = 0; e < N; e++) dw[k][e] = db[k][e] = 0.f;
     }
+    const float w1 = load_affine_one<T>(a.w, a.affine_f32, last, tail, 1.0f);
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
+    int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
+    typename Pack<T>::type next_x[NV], next_dy[NV];
+    T next_x1, next_dy1;
+    float next_mean, next_r;
+    const auto ask = [&](int64_t i) {
+        const T *x = static_cast<const T *>(a.x) + i * a.x_stride, *dy = static_cast<const T *>(a.dy) + i * a.dy_stride;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            next_x[k] = next_dy[k] = {};
+            if (i < a.rows && k * TPR + t < packs) {
+                next_x[k] = load_pack<STREAM>(x + (k * TPR + t) * N);
+                next_dy[k] = load_pack<STREAM>(dy + (k * TPR + t) * N);
+            }
+        }
+        next_x1 = next_dy1 = T(0);
+        if (i < a.rows && tail) { next_x1 = x[last]; next_dy1 = dy[last]; }
+        next_mean = i < a.rows ? a.mean[i] : 0.f;
+        next_r = i < a.rows ? a.rstd[i] : 0.f;
+    };
+    ask(row);
     int turn = 0;
-    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
-        const int64_t row = first + threadIdx.x / TPR;
-        const bool in = row < a.rows;
-        const int64_t cols = in ? a.cols : 0, at = in ? row : 0;
-        const T *x = static_cast<const T *>(a.x) + at * a.x_stride, *dy = static_cast<const T *>(a.dy) + at * a.dy_stride;
-        const float mean = a.mean[at], r = a.rstd[at];
-        float4 h[NV], g[NV];
-        float s[2] = {0.f, 0.f};
+    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += step, row += step, turn ^= 1) {
+        const float mean = next_mean, r = next_r;
+        const float h1 = ((float)next_x1 - mean) * r;
+        float h[NV][N], g[NV][N], g1 = (float)next_dy1;
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            h[k] = load4(x, (int64_t)(k * TPR + t) * 4, cols);
-            g[k] = load4(dy, (int64_t)(k * TPR + t) * 4, cols);
-        }
+        for (int k = 0; k < NV; k++)
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int64_t c = (int64_t)(k * TPR + t) * 4;
-            // h of an element past the row's end is 0, not -mean * r, which could be infinite
-            h[k].x = c < cols ? (h[k].x - mean) * r : 0.f;
-            h[k].y = c + 1 < cols ? (h[k].y - mean) * r : 0.f;
-            h[k].z = c + 2 < cols ? (h[k].z - mean) * r : 0.f;
-            h[k].w = c + 3 < cols ? (h[k].w - mean) * r : 0.f;
-            dw[k].x += g[k].x * h[k].x; dw[k].y += g[k].y * h[k].y; dw[k].z += g[k].z * h[k].z; dw[k].w += g[k].w * h[k].w;
-            db[k].x += g[k].x; db[k].y += g[k].y; db[k].z += g[k].z; db[k].w += g[k].w;
-            g[k].x *= w[k].x; g[k].y *= w[k].y; g[k].z *= w[k].z; g[k].w *= w[k].w;
-            s[0] += sum4(g[k]);
-            s[1] += (g[k].x * h[k].x + g[k].y * h[k].y) + (g[k].z * h[k].z + g[k].w * h[k].w);
-        }
+            for (int e = 0; e < N; e++) { h[k][e] = ((float)next_x[k][e] - mean) * r; g[k][e] = (float)next_dy[k][e]; }
+        if (first + step < a.rows) ask(row + step);
+        dw1 += g1 * h1;
+        db1 += g1;
+        g1 *= w1;
+        float s[2] = {g1, g1 * h1};
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                dw[k][e] += g[k][e] * h[k][e];
+                db[k][e] += g[k][e];
+                g[k][e] *= w[k][e];
+                s[0] += g[k][e];
+                s[1] += g[k][e] * h[k][e];
+            }
         if (!a.dx) continue;
         group_sum<TPR>(s, cell, turn);
         const float m0 = s[0] * inv, m1 = s[1] * inv;
-        T *dx = static_cast<T *>(a.dx) + at * a.dx_stride;
+        if (row < a.rows) {
+            T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
-            store4(dx, (int64_t)(k * TPR + t) * 4, cols,
-                   make_float4(r * (g[k].x - m0 - h[k].x * m1), r * (g[k].y - m0 - h[k].y * m1), r * (g[k].z - m0 - h[k].z * m1), r * (g[k].w - m0 - h[k].w * m1)));
+            for (int k = 0; k < NV; k++) {
+#pragma unroll
+                for (int e = 0; e < N; e++) g[k][e] = r * (g[k][e] - m0 - h[k][e] * m1);
+                if (k * TPR + t < packs) store_pack(dx + (k * TPR + t) * N, g[k], a.stream);
+            }
+            if (tail) dx[last] = (T)(r * (g1 - m0 - h1 * m1));
+        }
     }
     if (!a.part) return;
 #pragma unroll
@@ -212,16 +306,30 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(AZ_NORM_THRE
         float *part = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.cols;
         if constexpr (GROUPS == 1) {
 #pragma unroll
-            for (int k = 0; k < NV; k++) store4(part, (int64_t)(k * TPR + t) * 4, a.cols, which ? db[k] : dw[k]);
+            for (int k = 0; k < NV; k++) {
+                const float *f = which ? db[k] : dw[k];
+                if (k * TPR + t < packs) {
+#pragma unroll
+                    for (int e = 0; e < N; e += 4) store4(part + (k * TPR + t) * N + e, make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]));
+                }
+            }
+            if (tail) part[last] = which ? db1 : dw1;
         } else {
             __syncthreads();
+            float *mine = gather + (threadIdx.x / TPR) * WIDTH;
 #pragma unroll
-            for (int k = 0; k < NV; k++) gather[(threadIdx.x / TPR) * (WIDTH / 4) + k * TPR + t] = which ? db[k] : dw[k];
+            for (int k = 0; k < NV; k++) {
+                if (k * TPR + t < packs) {
+#pragma unroll
+                    for (int e = 0; e < N; e++) mine[(k * TPR + t) * N + e] = which ? db[k][e] : dw[k][e];
+                }
+            }
+            if (tail) mine[last] = which ? db1 : dw1;
             __syncthreads();
-            for (int c = threadIdx.x; c < a.cols; c += AZ_NORM_THREADS) {
+            for (int c = threadIdx.x; c < cols; c += THREADS) {
                 float sum = 0.f;
 #pragma unroll
-                for (int g = 0; g < GROUPS; g++) sum += reinterpret_cast<const float *>(gather)[g * WIDTH + c];
+                for (int i = 0; i < GROUPS; i++) sum += gather[i * WIDTH + c];
                 part[c] = sum;
             }
         }
@@ -258,9 +366,9 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
 }
 
 // The sums over rows for wide rows: a workgroup takes 1024 columns and every gridDim.y-th row.
-template <typename T> __global__ __launch_bounds__(AZ_NORM_THREADS) void k_layer_norm_cols_wide(NormBwd a)
+template <typename T> __global__ __launch_bounds__(AZ_NORM_COLS_WIDE_THREADS) void k_layer_norm_cols_wide(NormBwd a)
 {
-    const int64_t c = ((int64_t)blockIdx.x * AZ_NORM_THREADS + threadIdx.x) * 4;
+    const int64_t c = ((int64_t)blockIdx.x * AZ_NORM_COLS_WIDE_THREADS + threadIdx.x) * 4;
     if (c >= a.cols) return;
     float4 dw = make_float4(0.f, 0.f, 0.f, 0.f), db = dw;
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -274,21 +382,25 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_THREADS) void k_layer
     store4(a.part + ((int64_t)gridDim.y + blockIdx.y) * a.cols, c, a.cols, db);
 }
 
-// Adds the workgroups' sums: 64 columns per workgroup, its 16 waves take every 16th part and meet in LDS.  blockIdx.y: dw, db.
+// Adds the workgroups' sums.  16 columns per workgroup, so that even a row of 256 columns gives 32 of them: each row of 16 lanes
+// takes every 64th part, the four rows of a wave add up by row swaps, the 16 waves in LDS.  blockIdx.y: dw, db.
 template <typename T> __global__ __launch_bounds__(1024) void k_layer_norm_cols(const float *part, int64_t parts, int64_t cols, void *dw, void *db, bool affine_f32)
 {
-    __shared__ float cell[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    __shared__ float cell[16][16];
+    const int lane = threadIdx.x & 15, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 16 + lane;
     void *out = blockIdx.y ? db : dw;
     if (!out) return;
     part += (int64_t)blockIdx.y * parts * cols;
     float s = 0.f;
-    if (c < cols)
-        for (int64_t p = wave; p < parts; p += 16) s += part[p * cols + c];
-    cell[wave][lane] = s;
+    if (c < cols) {
+#pragma unroll 8
+        for (int64_t p = threadIdx.x >> 4; p < parts; p += 64) s += part[p * cols + c];
+    }
+    s = add_halves(add_row_pairs(s));
+    if ((threadIdx.x & 63) < 16) cell[wave][lane] = s;
     __syncthreads();
-    if (wave || c >= cols) return;
+    if (threadIdx.x >= 16 || c >= cols) return;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; i++) s += cell[i][lane];

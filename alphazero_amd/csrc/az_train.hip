@@ -31,23 +31,62 @@ int fail_hip(const char *what, hipError_t e)
     return az_fail(AZ_ERR_HIP, buf);
 }
 
-// Workgroups that keep the chip's memory busy when each walks over many rows: eight of 256 threads fit a compute unit at once.
-int64_t resident_blocks() { return 256 * 8; }
-
 bool bad_type(int32_t t) { return t != AZ_TYPE_F32 && t != AZ_TYPE_BF16 && t != AZ_TYPE_F16; }
 
-// threads per row and register groups per thread: the narrowest form that holds the row
-#define AZ_NORM_MAX_COLS 8192
-template <typename T, typename Launch> void norm_form(int64_t cols, const Launch &launch)
+// Whole 16-byte packs of a row.  The register forms hold up to 8192 elements in them, 8 to a thread of the largest workgroup
+// (16 would spill in the backward pass, which holds five numbers for each).
+int64_t norm_packs(int64_t cols, int32_t type) { return cols / (type == AZ_TYPE_F32 ? 4 : 8); }
+bool norm_wide(int64_t cols, int32_t type) { return norm_packs(cols, type) > (type == AZ_TYPE_F32 ? 2048 : 1024); }
+
+// Threads per row and packs per thread: the narrowest form that holds the row, one wave up to 256 packs.
+template <typename T, typename Launch> void norm_form(int64_t packs, const Launch &launch)
 {
-    if (cols <= 64) launch.template operator()<T, 16, 1>();
-    else if (cols <= 256) launch.template operator()<T, 64, 1>();
-    else if (cols <= 512) launch.template operator()<T, 64, 2>();
-    else if (cols <= 1024) launch.template operator()<T, 64, 4>();
-    else if (cols <= 2048) launch.template operator()<T, 256, 2>();
-    else if (cols <= 4096) launch.template operator()<T, 256, 4>();
-    else launch.template operator()<T, 256, 8>();
+    constexpr int NV = sizeof(T) == 4 ? 2 : 1;   // packs of 8 elements
+    if (packs <= 16) launch.template operator()<T, 16, 1>();
+    else if (packs <= 32) launch.template operator()<T, 32, 1>();
+    else if (packs <= 64) launch.template operator()<T, 64, 1>();
+    else if (packs <= 128) launch.template operator()<T, 64, 2>();
+    else if (packs <= 256) launch.template operator()<T, 64, 4>();
+    else if (packs <= 512) launch.template operator()<T, 512 / NV, NV>();
+    else if (packs <= 1024) launch.template operator()<T, 1024 / NV, NV>();
+    else if constexpr (NV == 2) launch.template operator()<T, 1024, 2>();
 }
+
+// rows that a workgroup works on at a time, and its threads, by the same rule
+int64_t norm_groups(int64_t packs) { return packs <= 16 ? 16 : packs <= 32 ? 8 : packs <= 256 ? 4 : 1; }
+int64_t norm_block(int64_t packs, int32_t type)
+{
+    const int64_t nv = type == AZ_TYPE_F32 ? 2 : 1;
+    return packs <= 256 * nv ? 256 : packs <= 512 * nv ? 512 : 1024;
+}
+
+// Workgroups of a pass over many rows, each of which walks over its share of them.  More than the memory needs in flight only
+// spread the accesses: rows of 256 float32 (whole cache lines) take 65 us with 1024 workgroups forward and 71 with 2048
+// (185 k rows), 100 us backward with 768 and 107 with 1024.  Rows that end inside a line wait for each other's lines and want
+// more: 361 16-bit columns, 100 k rows: 34 us with 2048 and 38 with 1024; backward 43 with 1024 and 48 with 768.  Forms with a
+// workgroup to a row wait at its barriers and want all that fit (1500 16-bit columns: 32 us with 1024, 47 with 512).
+bool norm_lines(int64_t cols, int32_t type) { return cols * (type == AZ_TYPE_F32 ? 4 : 2) % 128 == 0; }
+
+int64_t norm_fwd_blocks(int64_t cols, int32_t type)
+{
+    const int64_t packs = norm_packs(cols, type);
+    if (packs > 256) return 256 * 2048 / norm_block(packs, type);
+    if (packs > 128 && type != AZ_TYPE_F32) return 768;   // (as many as its registers leave room for)
+    return norm_lines(cols, type) ? 1024 : 2048;
+}
+
+int64_t norm_bwd_blocks(int64_t cols, int32_t type)
+{
+    const int64_t packs = norm_packs(cols, type);
+    if (packs <= 64) return norm_lines(cols, type) ? 768 : 1024;
+    if (packs <= 128) return 768;
+    if (packs <= 256) return type == AZ_TYPE_F32 ? 512 : 256;
+    return packs <= 512 ? 512 : 256;
+}
+
+// Of the eight L2 caches together.  What is larger is written, and read for the last time, past them: 361 16-bit columns, 100 k
+// rows, backward 43 us against 46; 256 float32 columns, 92 k rows, forward 32 against 36.
+#define AZ_L2_BYTES (32 << 20)
 
 template <typename Launch> void by_type(int32_t type, const Launch &launch)
 {
@@ -57,54 +96,56 @@ template <typename Launch> void by_type(int32_t type, const Launch &launch)
 }
 
 struct FwdForm {
-    const NormFwd &a; hipStream_t st;
+    const NormFwd &a; hipStream_t st; int64_t packs; int32_t type;
     template <typename T, int TPR, int NV> void operator()() const
     {
-        const int64_t groups = AZ_NORM_THREADS / TPR, blocks = (a.rows + groups - 1) / groups;
-        k_layer_norm_fwd<T, TPR, NV><<<(unsigned)std::min(blocks, resident_blocks()), AZ_NORM_THREADS, 0, st>>>(a);
+        const int64_t groups = norm_groups(packs), blocks = (a.rows + groups - 1) / groups;
+        k_layer_norm_fwd<T, TPR, NV><<<(unsigned)std::min(blocks, norm_fwd_blocks(a.cols, type)), norm_threads(TPR), 0, st>>>(a);
     }
 };
 struct FwdType {
-    const NormFwd &a; hipStream_t st;
+    const NormFwd &a; hipStream_t st; int32_t type;
     template <typename T> void operator()() const
     {
-        if (a.cols > AZ_NORM_MAX_COLS) k_layer_norm_fwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2 * 256), AZ_NORM_WIDE_THREADS, 0, st>>>(a);
-        else norm_form<T>(a.cols, FwdForm{a, st});
+        if (norm_wide(a.cols, type)) k_layer_norm_fwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2 * 256), AZ_NORM_WIDE_THREADS, 0, st>>>(a);
+        else norm_form<T>(norm_packs(a.cols, type), FwdForm{a, st, norm_packs(a.cols, type), type});
     }
 };
 
 // Workgroups of the backward pass, each of which leaves one row of partial sums: a function of the sizes alone, so the order
-// of the sums is the same on every call.
-int64_t bwd_parts(int64_t rows, int64_t cols)
+// of the sums is the same on every call.  Four rows or more for each group of threads where there are rows enough, since
+// every workgroup costs a row of sums written and read again.
+int64_t bwd_parts(int64_t rows, int64_t cols, int32_t type)
 {
     if (rows <= 0) return 0;
-    if (cols > AZ_NORM_MAX_COLS) return std::min<int64_t>(rows, 64);
-    const int64_t groups = cols <= 64 ? 16 : cols <= 1024 ? 4 : 1;
-    return std::min<int64_t>((rows + groups - 1) / groups, 1024);
+    if (norm_wide(cols, type)) return std::min<int64_t>(rows, 64);
+    const int64_t packs = norm_packs(cols, type), groups = norm_groups(packs), each = (rows + groups - 1) / groups;
+    return std::min(norm_bwd_blocks(cols, type), std::max((each + 3) / 4, std::min<int64_t>(each, 64)));
 }
 
 struct BwdForm {
-    const NormBwd &a; hipStream_t st;
+    const NormBwd &a; hipStream_t st; int64_t parts;
     template <typename T, int TPR, int NV> void operator()() const
     {
-        k_layer_norm_bwd<T, TPR, NV><<<(unsigned)bwd_parts(a.rows, a.cols), AZ_NORM_THREADS, 0, st>>>(a);
+        if (a.stream) k_layer_norm_bwd<T, TPR, NV, true><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
+        else k_layer_norm_bwd<T, TPR, NV, false><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
     }
 };
 struct BwdType {
-    const NormBwd &a; void *dw, *db; hipStream_t st;
+    const NormBwd &a; void *dw, *db; hipStream_t st; int32_t type;
     template <typename T> void operator()() const
     {
-        const int64_t parts = bwd_parts(a.rows, a.cols);
+        const int64_t parts = bwd_parts(a.rows, a.cols, type);
         if (parts > 0) {
-            if (a.cols > AZ_NORM_MAX_COLS) {
+            if (norm_wide(a.cols, type)) {
                 if (a.dx) k_layer_norm_bwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2 * 256), AZ_NORM_WIDE_THREADS, 0, st>>>(a);
-                if (a.part) k_layer_norm_cols_wide<T><<<dim3((unsigned)((a.cols + 1023) / 1024), (unsigned)parts), AZ_NORM_THREADS, 0, st>>>(a);
+                if (a.part) k_layer_norm_cols_wide<T><<<dim3((unsigned)((a.cols + 1023) / 1024), (unsigned)parts), AZ_NORM_COLS_WIDE_THREADS, 0, st>>>(a);
             } else {
-                norm_form<T>(a.cols, BwdForm{a, st});
+                norm_form<T>(norm_packs(a.cols, type), BwdForm{a, st, parts});
             }
         }
         if (dw || db)
-            k_layer_norm_cols<T><<<dim3((unsigned)((a.cols + 63) / 64), 2), 1024, 0, st>>>(a.part, parts, a.cols, dw, db, a.affine_f32);
+            k_layer_norm_cols<T><<<dim3((unsigned)((a.cols + 15) / 16), 2), 1024, 0, st>>>(a.part, parts, a.cols, dw, db, a.affine_f32);
     }
 };
 
@@ -130,15 +171,16 @@ extern "C" int az_layer_norm_fwd_dev(int32_t device, void *stream, int32_t type,
     if (x_stride < 0 || (y_stride < cols && rows > 1)) return az_fail(AZ_ERR_ARG, "layer norm: bad row stride");
     DeviceScope scope(device);
     if (scope.error != hipSuccess) return fail_hip("layer norm: device", scope.error);
-    const NormFwd a{x, weight, bias, y, mean, rstd, rows, cols, x_stride, y_stride, (float)eps, affine_type == AZ_TYPE_F32};
-    by_type(type, FwdType{a, static_cast<hipStream_t>(stream)});
+    const NormFwd a{x, weight, bias, y, mean, rstd, rows, cols, x_stride, y_stride, (float)eps, affine_type == AZ_TYPE_F32,
+                    rows * cols * (type == AZ_TYPE_F32 ? 4 : 2) > AZ_L2_BYTES};
+    by_type(type, FwdType{a, static_cast<hipStream_t>(stream), type});
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? AZ_OK : fail_hip("layer norm", e);
 }
 
-extern "C" int64_t az_layer_norm_bwd_workspace(int64_t rows, int64_t cols)
+extern "C" int64_t az_layer_norm_bwd_workspace(int32_t type, int64_t rows, int64_t cols)
 {
-    return rows < 0 || cols < 1 ? 0 : 2 * bwd_parts(rows, cols) * cols;
+    return rows < 0 || cols < 1 || bad_type(type) ? 0 : 2 * bwd_parts(rows, cols, type) * cols;
 }
 
 extern "C" int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, const void *dy, int64_t dy_stride,
@@ -150,13 +192,14 @@ extern "C" int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type,
     if (rows > 0 && (!dy || !x || !mean || !rstd)) return az_fail(AZ_ERR_ARG, "layer norm backward: null array");
     if (dy_stride < 0 || x_stride < 0 || (dx && dx_stride < cols && rows > 1)) return az_fail(AZ_ERR_ARG, "layer norm backward: bad row stride");
     const bool sums = dweight || dbias;
-    const int64_t need = az_layer_norm_bwd_workspace(rows, cols);
+    const int64_t need = az_layer_norm_bwd_workspace(type, rows, cols);
     if (sums && need > 0 && (!workspace || workspace_floats < need)) return az_fail(AZ_ERR_ARG, "layer norm backward: workspace smaller than az_layer_norm_bwd_workspace");
     if (!dx && !sums) return AZ_OK;
     DeviceScope scope(device);
     if (scope.error != hipSuccess) return fail_hip("layer norm backward: device", scope.error);
-    const NormBwd a{dy, x, weight, mean, rstd, dx, sums ? workspace : nullptr, rows, cols, dy_stride, x_stride, dx_stride, affine_type == AZ_TYPE_F32};
-    by_type(type, BwdType{a, dweight, dbias, static_cast<hipStream_t>(stream)});
+    const NormBwd a{dy, x, weight, mean, rstd, dx, sums ? workspace : nullptr, rows, cols, dy_stride, x_stride, dx_stride,
+                    affine_type == AZ_TYPE_F32, rows * cols * (type == AZ_TYPE_F32 ? 4 : 2) > AZ_L2_BYTES};
+    by_type(type, BwdType{a, dweight, dbias, static_cast<hipStream_t>(stream), type});
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? AZ_OK : fail_hip("layer norm backward", e);
 }
@@ -236,7 +279,7 @@ int adamw_step(int32_t device, void *stream, int64_t tensors, void *const *param
     k.decay = (float)(lr * weight_decay);
     k.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     k.inv_sqrt_c2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
-    k.eps = (float)eps;
+    k.eps = eps > 0.0 ? std::max((float)eps, 1.17549435e-38f) : 0.f;   // (subnormal numbers do not survive the reciprocal)
     const int turns = total <= ((int64_t)1 << 20) ? 1 : 2;
     const int64_t chunk = turns * 4 * AZ_ADAMW_THREADS;
     AdamwTable t;

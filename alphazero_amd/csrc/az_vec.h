@@ -42,6 +42,31 @@ template <typename T> __device__ __forceinline__ void store4(T *p, int64_t i, in
     if (i + 2 < n) p[i + 2] = (T)f.z;
 }
 
+// As many neighbouring elements as one 16-byte access holds (4 of float32, 8 of 16 bits), as they lie in memory.
+template <typename T> struct Pack {
+    static constexpr int N = 16 / sizeof(T);
+    typedef T type __attribute__((ext_vector_type(N)));
+    typedef type any __attribute__((aligned(alignof(T))));   // at any element's address
+};
+
+// STREAM: what will not be read again from the L2 cache leaves room there for what will.
+template <bool STREAM, typename T> __device__ __forceinline__ typename Pack<T>::type load_pack(const T *p)
+{
+    const typename Pack<T>::any *from = reinterpret_cast<const typename Pack<T>::any *>(p);
+    if constexpr (STREAM) return __builtin_nontemporal_load(from);
+    else return *from;
+}
+
+template <typename T> __device__ __forceinline__ void store_pack(T *p, const float (&f)[Pack<T>::N], bool stream)
+{
+    typename Pack<T>::type out;
+#pragma unroll
+    for (int e = 0; e < Pack<T>::N; e++) out[e] = (T)f[e];
+    typename Pack<T>::any *to = reinterpret_cast<typename Pack<T>::any *>(p);
+    if (stream) __builtin_nontemporal_store(out, to);
+    else *to = out;
+}
+
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_row(uint32_t x)
 {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
@@ -59,14 +84,22 @@ __device__ __forceinline__ float row16_sum(float x)
     return x;
 }
 
-__device__ __forceinline__ float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
-
-// Sum over a wave's 64 lanes, in every lane; needs all lanes active.
-__device__ __forceinline__ float wave_sum(float x)
+// gfx950's row swaps hand every lane the values of both rows (or both halves) of a pair, in the same order: what is added up
+// from them has the same bits in all lanes.
+__device__ __forceinline__ float add_row_pairs(float x)     // lane i of rows 2j and 2j+1: x of row 2j + x of row 2j+1
 {
-    x = row16_sum(x);
-    return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+__device__ __forceinline__ float add_halves(float x)        // lane i of both halves of the wave
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Sum over groups of 32 neighbouring lanes / over a wave's 64, in every lane; needs all lanes active.
+__device__ __forceinline__ float half_sum(float x) { return add_row_pairs(row16_sum(x)); }
+__device__ __forceinline__ float wave_sum(float x) { return add_halves(half_sum(x)); }
 
 // Largest of 64 unsigned values, in every lane; needs all lanes active.
 __device__ __forceinline__ uint32_t wave_umax(uint32_t x)

@@ -71,7 +71,7 @@ class _LayerNorm(torch.autograd.Function):
         dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_x else None
         dw = torch.empty(cols, dtype=ctx.affine_dtype, device=device) if want_w else None
         db = torch.empty(cols, dtype=ctx.affine_dtype, device=device) if want_b else None
-        n = L.az_layer_norm_bwd_workspace(rows, cols) if want_w or want_b else 0
+        n = L.az_layer_norm_bwd_workspace(TYPE_IDS[x.dtype], rows, cols) if want_w or want_b else 0
         space = torch.empty(n, dtype=torch.float32, device=device) if n else None
         w = weight.contiguous() if weight is not None else None
         at = stats.data_ptr()

@@ -346,9 +346,9 @@ int az_layer_norm_fwd_dev(int32_t device, void *stream, int32_t type, int32_t af
                           const void *x, int64_t x_stride, const void *weight, const void *bias, void *y, int64_t y_stride,
                           float *mean, float *rstd);
 /* Its gradient: dx (of x's type), dweight and dbias (of affine_type, sums over the rows, the same bits on every call); each may
- * be NULL if not wanted.  workspace: az_layer_norm_bwd_workspace(rows, cols) floats, needed for dweight / dbias; it may be reused
+ * be NULL if not wanted.  workspace: az_layer_norm_bwd_workspace(type, rows, cols) floats, needed for dweight / dbias; it may be reused
  * as soon as the stream has passed the call. */
-int64_t az_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
+int64_t az_layer_norm_bwd_workspace(int32_t type, int64_t rows, int64_t cols);
 int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, const void *dy,
                           int64_t dy_stride, const void *x, int64_t x_stride, const void *weight, const float *mean, const float *rstd,
                           void *dx, int64_t dx_stride, void *dweight, void *dbias, float *workspace, int64_t workspace_floats);

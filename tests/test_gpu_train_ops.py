@@ -57,7 +57,7 @@ def _check_norm(x, w, b, dy, eps=1e-5):
 
 
 COLS = [1, 2, 3, 4, 5, 30, 63, 64, 65, 128, 255, 256, 257, 361, 511, 512, 513, 722, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192,
-        8193, 10001, 33000]
+        8193, 10001, 16383, 16384, 16385, 33000]
 
 
 @pytest.mark.parametrize("cols", COLS)
