@@ -38,9 +38,13 @@ __device__ __forceinline__ int adamw_tensor(const AdamwTable &a, uint32_t block)
     return __popcll(__ballot(last <= block));
 }
 
+// Square root and reciprocal by the instructions that are right to one step of float32, a third of the work of the correctly
+// rounded ones: their error is in the update, not in the weight.  They take no subnormal numbers, so a tiny v is scaled.
 __device__ __forceinline__ float adamw_weight(float w, float m, float v, const AdamwScalars &k)
 {
-    return w - k.decay * w - k.step_size * (m / (sqrtf(v) * k.inv_sqrt_c2 + k.eps));
+    const bool small = v < 0x1p-96f;
+    const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? k.inv_sqrt_c2 * 0x1p-32f : k.inv_sqrt_c2);
+    return w - k.decay * w - k.step_size * m * __builtin_amdgcn_rcpf(root + k.eps);
 }
 
 __device__ __forceinline__ void adamw_32(float &w, float g, float &m, float &v, const AdamwScalars &k)
@@ -50,30 +54,59 @@ __device__ __forceinline__ void adamw_32(float &w, float g, float &m, float &v, 
     w = adamw_weight(w, m, v, k);
 }
 
-// A workgroup takes TURNS * 1024 neighbouring elements of one tensor.
-template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_32(AdamwTable a, AdamwScalars k)
+// What a workgroup works on: TURNS * 1024 neighbouring elements of one tensor, `left` of them before its end.
+struct AdamwChunk {
+    int tensor;
+    int64_t first, left;
+};
+
+template <int TURNS> __device__ __forceinline__ AdamwChunk adamw_chunk(const AdamwTable &a)
 {
     const int i = __builtin_amdgcn_readfirstlane(adamw_tensor(a, blockIdx.x));
     const int64_t first = (int64_t)(blockIdx.x - (i ? a.last[i - 1] : 0u)) * (TURNS * 4 * AZ_ADAMW_THREADS);
-    const int64_t n = a.n[i];
-    T *wp = static_cast<T *>(a.param[i]);
-    const T *gp = static_cast<const T *>(a.grad[i]);
-    float *mp = static_cast<float *>(a.m[i]), *vp = static_cast<float *>(a.v[i]);
+    return AdamwChunk{i, first, a.n[i] - first};
+}
+
+// FULL: the chunk ends before its tensor does, so nothing needs a check
+template <bool FULL, typename T> __device__ __forceinline__ float4 load4(const T *p, int i, int n)
+{
+    if constexpr (FULL) return load4(p + i);
+    else return load4(p, (int64_t)i, (int64_t)n);
+}
+template <bool FULL, typename T> __device__ __forceinline__ void store4(T *p, int i, int n, float4 f)
+{
+    if constexpr (FULL) store4(p + i, f);
+    else store4(p, (int64_t)i, (int64_t)n, f);
+}
+
+template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adamw_32_chunk(const AdamwTable &a, const AdamwScalars &k, const AdamwChunk &c)
+{
+    T *wp = static_cast<T *>(a.param[c.tensor]) + c.first;
+    const T *gp = static_cast<const T *>(a.grad[c.tensor]) + c.first;
+    float *mp = static_cast<float *>(a.m[c.tensor]) + c.first, *vp = static_cast<float *>(a.v[c.tensor]) + c.first;
+    const int n = (int)min(c.left, (int64_t)(TURNS * 4 * AZ_ADAMW_THREADS));
     float4 w[TURNS], g[TURNS], m[TURNS], v[TURNS];
 #pragma unroll
     for (int u = 0; u < TURNS; u++) {
-        const int64_t at = first + (u * AZ_ADAMW_THREADS + threadIdx.x) * 4;
-        w[u] = load4(wp, at, n); g[u] = load4(gp, at, n); m[u] = load4(mp, at, n); v[u] = load4(vp, at, n);
+        const int at = (u * AZ_ADAMW_THREADS + threadIdx.x) * 4;
+        w[u] = load4<FULL>(wp, at, n); g[u] = load4<FULL>(gp, at, n); m[u] = load4<FULL>(mp, at, n); v[u] = load4<FULL>(vp, at, n);
     }
 #pragma unroll
     for (int u = 0; u < TURNS; u++) {
-        const int64_t at = first + (u * AZ_ADAMW_THREADS + threadIdx.x) * 4;
+        const int at = (u * AZ_ADAMW_THREADS + threadIdx.x) * 4;
         adamw_32(w[u].x, g[u].x, m[u].x, v[u].x, k);
         adamw_32(w[u].y, g[u].y, m[u].y, v[u].y, k);
         adamw_32(w[u].z, g[u].z, m[u].z, v[u].z, k);
         adamw_32(w[u].w, g[u].w, m[u].w, v[u].w, k);
-        store4(wp, at, n, w[u]); store4(mp, at, n, m[u]); store4(vp, at, n, v[u]);
+        store4<FULL>(wp, at, n, w[u]); store4<FULL>(mp, at, n, m[u]); store4<FULL>(vp, at, n, v[u]);
     }
+}
+
+template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_32(AdamwTable a, AdamwScalars k)
+{
+    const AdamwChunk c = adamw_chunk<TURNS>(a);
+    if (c.left >= TURNS * 4 * AZ_ADAMW_THREADS) adamw_32_chunk<T, TURNS, true>(a, k, c);
+    else adamw_32_chunk<T, TURNS, false>(a, k, c);
 }
 
 // ---- states in 8 bits -------------------------------------------------------------------------------------------------
@@ -84,46 +117,98 @@ template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) 
 // the top.  A code is the nearest one in the domain in which codes are evenly spaced, c = round(127 sqrt(|m| / S)),
 // c = round(255 (v / S)^(1/4)), and at least 1 where v > 0, so that no element is ever divided by eps alone because its
 // v was rounded away.
-// Means and codes are worked out in 64 bits: a value next to a border between two codes goes to the right side of it, and
-// the multiplications cost less than the memory they wait for.  Every operation of the means rounds by itself, in the order in
-// which the formulas are written (no fused multiply-add): b1 S + (1 - b1) g lies exactly between two float32 values in one
-// block of a hundred, and the scale must not depend on how a compiler contracts the sum.  The border is found by comparing powers, not by taking roots:
-// a float32 estimate is off by one at most, and (2c - 1)^2 S <= 254^2 |m| < (2c + 1)^2 S settles it.
+// Means are worked out in 64 bits, every operation rounded by itself in the order in which the formulas are written (no fused
+// multiply-add): b1 S + (1 - b1) g lies exactly between two float32 values in one block of a hundred, and the scale must not
+// depend on how a compiler contracts the sum.
+// Codes are those of the 64-bit means too: a value next to a border between two codes goes to the right side of it.  A
+// float32 estimate of 127 sqrt(|m| / S) or 255 (v / S)^(1/4) is off by less than 1e-4 (one step each of the conversion, the
+// reciprocal, two roots and the products), so only what it puts within 2e-4 of a border, one wave in eight, is compared with
+// that border, by powers and without roots: (2c - 1)^2 S <= 254^2 |m| < (2c + 1)^2 S.  With that, 95 M bfloat16 parameters take
+// 219 us (950 MB, 4.3 TB/s); with the comparison for every element they took 360 us and were bound by arithmetic.
 // A block with an infinity or a NaN in it has a scale that is not finite and reads back as NaN as a whole.
 
-__device__ __forceinline__ double dequantize_m(int c, double s) { return s * (double)(c * abs(c)) * (1.0 / 16129.0); }
+// byte e of a word as int8 / uint8, in float32: c |c| and c^2 are exact there
+__device__ __forceinline__ float signed_code(uint32_t w, int e) { return (float)(int8_t)(w >> (8 * e)); }
+__device__ __forceinline__ float unsigned_code(uint32_t w, int e) { return (float)(uint8_t)(w >> (8 * e)); }
 
-__device__ __forceinline__ double dequantize_v(int c, double s)
+__device__ __forceinline__ double dequantize_m(float c, double s) { return s * (double)(c * fabsf(c)) * (1.0 / 16129.0); }
+
+__device__ __forceinline__ double dequantize_v(float c, double s)
 {
     const double q = (double)(c * c);
     return s * (q * q) * (1.0 / 4228250625.0);   // 255^4
 }
 
-// s > 0 and finite, inv = 1 / s
-__device__ __forceinline__ int quantize_m(double m, double s, double inv)
+// the codes (as float32) from their borders; s > 0 and finite, inv = 1 / s
+__device__ __forceinline__ float border_m(double m, double s, double inv)
 {
     const double a = fabs(m), t = a * 64516.0;   // 254^2
     const int c = (int)rintf(127.0f * __builtin_amdgcn_sqrtf((float)(a * inv)));
     const double lo = (double)((2 * c - 1) * abs(2 * c - 1)) * s, hi = (double)((2 * c + 1) * (2 * c + 1)) * s;
-    const int r = min(c + (t >= hi ? 1 : 0) - (t < lo ? 1 : 0), 127);
-    return m < 0.0 ? -r : r;
+    return (float)min(c + (t >= hi ? 1 : 0) - (t < lo ? 1 : 0), 127);
 }
 
-__device__ __forceinline__ int quantize_v(double v, double s, double inv)
+__device__ __forceinline__ float border_v(double v, double s, double inv)
 {
     const double t = v * 67652010000.0;          // 510^4
     const int c = (int)rintf(255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)(v * inv))));
     const double l = (double)((2 * c - 1) * abs(2 * c - 1)), h = (double)((2 * c + 1) * (2 * c + 1));
-    const int r = min(c + (t >= h * h * s ? 1 : 0) - (t < l * fabs(l) * s ? 1 : 0), 255);
-    return v > 0.0 ? max(r, 1) : r;
+    return (float)min(c + (t >= h * h * s ? 1 : 0) - (t < l * fabs(l) * s ? 1 : 0), 255);
+}
+
+// four codes as the bytes of a word; `bits` are the scale's, the same in the whole wave
+__device__ __forceinline__ uint32_t quantize_m(const double (&m)[4], const float (&f)[4], uint32_t bits)
+{
+    if (bits == 0 || bits >= 0x7f800000u) return 0;
+    const float s = __uint_as_float(bits), inv = __builtin_amdgcn_rcpf(s);
+    bool near = s < 0x1p-100f || s > 0x1p100f;   // where the reciprocal is no longer a normal number, or close to it
+    float c[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float x = 127.0f * __builtin_amdgcn_sqrtf(fabsf(f[e]) * inv);
+        c[e] = rintf(x);
+        near |= fabsf(x - c[e]) > 0.4998f;
+    }
+    if (near) {
+        const double d = (double)s, dinv = 1.0 / d;
+#pragma unroll
+        for (int e = 0; e < 4; e++) c[e] = border_m(m[e], d, dinv);
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w = __builtin_amdgcn_cvt_pk_u8_f32(copysignf(c[e], f[e]) + 128.0f, e, w);
+    return w ^ 0x80808080u;
+}
+
+__device__ __forceinline__ uint32_t quantize_v(const double (&v)[4], const float (&f)[4], uint32_t bits)
+{
+    if (bits == 0 || bits >= 0x7f800000u) return 0;
+    const float s = __uint_as_float(bits), inv = __builtin_amdgcn_rcpf(s);
+    bool near = s < 0x1p-100f || s > 0x1p100f;
+    float c[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float x = 255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(f[e] * inv));
+        c[e] = rintf(x);
+        near |= fabsf(x - c[e]) > 0.4998f;
+    }
+    if (near) {
+        const double d = (double)s, dinv = 1.0 / d;
+#pragma unroll
+        for (int e = 0; e < 4; e++) c[e] = border_v(v[e], d, dinv);
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w = __builtin_amdgcn_cvt_pk_u8_f32(v[e] > 0.0 ? fmaxf(c[e], 1.0f) : 0.0f, e, w);
+    return w;
 }
 
 struct __attribute__((packed)) PackedWord { uint32_t v; };
 
 // four codes as one word (any address); those past the end are 0 / are not written
-__device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int64_t i, int64_t n)
+template <bool FULL> __device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int64_t i, int64_t n)
 {
-    if (i + 4 <= n) return reinterpret_cast<const PackedWord *>(p + i)->v;
+    if (FULL || i + 4 <= n) return reinterpret_cast<const PackedWord *>(p + i)->v;
     uint32_t w = 0;
     if (i < n) w = p[i];
     if (i + 1 < n) w |= (uint32_t)p[i + 1] << 8;
@@ -131,76 +216,75 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int64_t i, int6
     return w;
 }
 
-__device__ __forceinline__ void store_codes(uint8_t *p, int64_t i, int64_t n, uint32_t w)
+template <bool FULL> __device__ __forceinline__ void store_codes(uint8_t *p, int i, int n, uint32_t w)
 {
-    if (i + 4 <= n) { reinterpret_cast<PackedWord *>(p + i)->v = w; return; }
+    if (FULL || i + 4 <= n) { reinterpret_cast<PackedWord *>(p + i)->v = w; return; }
     if (i < n) p[i] = (uint8_t)w;
     if (i + 1 < n) p[i + 1] = (uint8_t)(w >> 8);
     if (i + 2 < n) p[i + 2] = (uint8_t)(w >> 16);
 }
 
-__device__ __forceinline__ uint32_t magnitude_bits(double x) { return __float_as_uint((float)x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// A workgroup takes TURNS * 1024 neighbouring elements of one tensor, each of its waves a block of 256 at a time.
-template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_8(AdamwTable a, AdamwScalars k)
+// A workgroup's chunk in blocks of 256, one for each of its waves at a time.
+template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adamw_8_chunk(const AdamwTable &a, const AdamwScalars &k, const AdamwChunk &ch)
 {
-    const int i = __builtin_amdgcn_readfirstlane(adamw_tensor(a, blockIdx.x));
-    const int64_t first = (int64_t)(blockIdx.x - (i ? a.last[i - 1] : 0u)) * (TURNS * 4 * AZ_ADAMW_THREADS);
-    const int64_t n = a.n[i];
-    T *wp = static_cast<T *>(a.param[i]);
-    const T *gp = static_cast<const T *>(a.grad[i]);
-    uint8_t *mp = static_cast<uint8_t *>(a.m[i]), *vp = static_cast<uint8_t *>(a.v[i]);
-    float *msp = a.m_scale[i], *vsp = a.v_scale[i];
+    T *wp = static_cast<T *>(a.param[ch.tensor]) + ch.first;
+    const T *gp = static_cast<const T *>(a.grad[ch.tensor]) + ch.first;
+    uint8_t *mp = static_cast<uint8_t *>(a.m[ch.tensor]) + ch.first, *vp = static_cast<uint8_t *>(a.v[ch.tensor]) + ch.first;
+    float *msp = a.m_scale[ch.tensor] + ch.first / AZ_ADAMW_BLOCK, *vsp = a.v_scale[ch.tensor] + ch.first / AZ_ADAMW_BLOCK;
+    const int n = (int)min(ch.left, (int64_t)(TURNS * 4 * AZ_ADAMW_THREADS));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    static_assert(AZ_ADAMW_THREADS * 4 == 4 * AZ_ADAMW_BLOCK, "four waves, a block each");
     float4 w[TURNS], g[TURNS];
     uint32_t mc[TURNS], vc[TURNS];
     float ms[TURNS], vs[TURNS];
 #pragma unroll
     for (int u = 0; u < TURNS; u++) {
-        const int64_t at = first + (u * AZ_ADAMW_THREADS + threadIdx.x) * 4;
-        w[u] = load4(wp, at, n); g[u] = load4(gp, at, n);
-        mc[u] = load_codes(mp, at, n); vc[u] = load_codes(vp, at, n);
-        const int64_t block = (at - (threadIdx.x & 63) * 4) / AZ_ADAMW_BLOCK;
-        const bool in = block * AZ_ADAMW_BLOCK < n;
+        const int at = (u * AZ_ADAMW_THREADS + threadIdx.x) * 4, block = u * 4 + wave;
+        w[u] = load4<FULL>(wp, at, n); g[u] = load4<FULL>(gp, at, n);
+        mc[u] = load_codes<FULL>(mp, at, n); vc[u] = load_codes<FULL>(vp, at, n);
+        const bool in = FULL || block * AZ_ADAMW_BLOCK < n;
         ms[u] = in ? msp[block] : 0.f; vs[u] = in ? vsp[block] : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < TURNS; u++) {
-        const int64_t at = first + (u * AZ_ADAMW_THREADS + threadIdx.x) * 4;
+        const int at = (u * AZ_ADAMW_THREADS + threadIdx.x) * 4, block = u * 4 + wave;
         float *we = reinterpret_cast<float *>(&w[u]);
         const float *ge = reinterpret_cast<const float *>(&g[u]);
         double m[4], v[4];
+        float mf[4], vf[4];
         uint32_t mb = 0, vb = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
 #pragma clang fp contract(off)
             const double gd = (double)ge[e];
-            m[e] = k.beta1 * dequantize_m((int8_t)(mc[u] >> (8 * e)), (double)ms[u]) + k.one_minus_beta1 * gd;
-            v[e] = k.beta2 * dequantize_v((uint8_t)(vc[u] >> (8 * e)), (double)vs[u]) + k.one_minus_beta2 * (gd * gd);
-            mb = max(mb, magnitude_bits(m[e]));
-            vb = max(vb, magnitude_bits(v[e]));
-            we[e] = adamw_weight(we[e], (float)m[e], (float)v[e], k);
+            m[e] = k.beta1 * dequantize_m(signed_code(mc[u], e), (double)ms[u]) + k.one_minus_beta1 * gd;
+            v[e] = k.beta2 * dequantize_v(unsigned_code(vc[u], e), (double)vs[u]) + k.one_minus_beta2 * (gd * gd);
+            mf[e] = (float)m[e];
+            vf[e] = (float)v[e];
+            mb = max(mb, magnitude_bits(mf[e]));
+            vb = max(vb, magnitude_bits(vf[e]));
         }
+#pragma unroll
+        for (int e = 0; e < 4; e++) we[e] = adamw_weight(we[e], mf[e], vf[e], k);
         // NaN has the largest magnitude bits of all, so the integer maximum keeps it
         mb = wave_umax(mb); vb = wave_umax(vb);
-        uint32_t mw = 0, vw = 0;
-        if (mb != 0 && mb < 0x7f800000u) {
-            const double s = (double)__uint_as_float(mb), inv = 1.0 / s;
-#pragma unroll
-            for (int e = 0; e < 4; e++) mw |= (uint32_t)(uint8_t)quantize_m(m[e], s, inv) << (8 * e);
-        }
-        if (vb != 0 && vb < 0x7f800000u) {
-            const double s = (double)__uint_as_float(vb), inv = 1.0 / s;
-#pragma unroll
-            for (int e = 0; e < 4; e++) vw |= (uint32_t)quantize_v(v[e], s, inv) << (8 * e);
-        }
-        store4(wp, at, n, w[u]);
-        store_codes(mp, at, n, mw); store_codes(vp, at, n, vw);
-        const int64_t start = at - (threadIdx.x & 63) * 4;
-        if ((threadIdx.x & 63) == 0 && start < n) {
-            msp[start / AZ_ADAMW_BLOCK] = __uint_as_float(mb);
-            vsp[start / AZ_ADAMW_BLOCK] = __uint_as_float(vb);
+        const uint32_t mw = quantize_m(m, mf, mb), vw = quantize_v(v, vf, vb);
+        store4<FULL>(wp, at, n, w[u]);
+        store_codes<FULL>(mp, at, n, mw); store_codes<FULL>(vp, at, n, vw);
+        if ((threadIdx.x & 63) == 0 && (FULL || block * AZ_ADAMW_BLOCK < n)) {
+            msp[block] = __uint_as_float(mb);
+            vsp[block] = __uint_as_float(vb);
         }
     }
+}
+
+template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_8(AdamwTable a, AdamwScalars k)
+{
+    const AdamwChunk c = adamw_chunk<TURNS>(a);
+    if (c.left >= TURNS * 4 * AZ_ADAMW_THREADS) adamw_8_chunk<T, TURNS, true>(a, k, c);
+    else adamw_8_chunk<T, TURNS, false>(a, k, c);
 }
 
 // the values that codes stand for, rounded once to float32
@@ -208,12 +292,12 @@ template <bool SIGNED> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_deq
 {
     const int64_t step = (int64_t)gridDim.x * AZ_ADAMW_THREADS * 4;
     for (int64_t at = ((int64_t)blockIdx.x * AZ_ADAMW_THREADS + threadIdx.x) * 4; at < n; at += step) {
-        const uint32_t w = load_codes(codes, at, n);
+        const uint32_t w = load_codes<false>(codes, at, n);
         const double s = (double)scales[at / AZ_ADAMW_BLOCK];
         float f[4];
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            f[e] = (float)(SIGNED ? dequantize_m((int8_t)(w >> (8 * e)), s) : dequantize_v((uint8_t)(w >> (8 * e)), s));
+            f[e] = (float)(SIGNED ? dequantize_m(signed_code(w, e), s) : dequantize_v(unsigned_code(w, e), s));
         store4(out, at, n, make_float4(f[0], f[1], f[2], f[3]));
     }
 }
