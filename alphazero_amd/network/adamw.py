@@ -12,17 +12,11 @@ itself uses the new means before they are rounded to codes.  A block that holds 
 
 Tensors on the GPU go through the kernel, on PyTorch's current stream; tensors on the CPU take the same formulas in PyTorch.
 """
-import ctypes as C
-from operator import attrgetter
-
 import torch
 
-from .device_ops import TYPE_IDS, check, current_stream, dense, in_memory_order, library
+from .device_ops import TYPES, binding, check, dense, in_memory_order
 
 STATE_BLOCK = 256   # AZ_STATE_BLOCK of include/az_engine.h
-
-_dtype, _shape, _numel, _pointer = attrgetter("dtype"), attrgetter("shape"), torch.Tensor.numel, torch.Tensor.data_ptr
-_contiguous, _device = torch.Tensor.is_contiguous, torch.Tensor.get_device
 
 
 def _blocks(n):
@@ -80,31 +74,8 @@ def dequantize_state(codes, scales):
     if codes.device.type != "cuda":
         in_memory_order(out).copy_(_values64(codes, scales))
         return out
-    device = codes.device.index
-    check(library().az_dequantize_state_dev(device, current_stream(device), codes.data_ptr(), scales.data_ptr(), codes.numel(),
-                                            int(codes.dtype == torch.int8), out.data_ptr()))
+    check(binding().dequantize_state(codes, scales, out))
     return out
-
-
-def _scalars(step, lr, betas, eps, weight_decay):
-    beta1, beta2 = betas
-    if isinstance(lr, torch.Tensor) or isinstance(step, torch.Tensor):
-        raise TypeError("lr and step are Python numbers")
-    if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0):
-        raise ValueError("lr, eps and weight_decay must not be negative")
-    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
-        raise ValueError("betas must lie in [0, 1)")
-    if step < 1:
-        raise ValueError("steps are counted from 1")
-
-
-def _laid_out_as(p, t, what):
-    if not (p.is_contiguous() and t.is_contiguous()) and (not dense(p) or p.stride() != t.stride()):
-        raise ValueError("%s does not lie in memory as its parameter does (or the parameter is not dense)" % what)
-
-
-def _pointers(tensors):
-    return (C.c_void_p * len(tensors))(*map(_pointer, tensors))
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
@@ -115,55 +86,14 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     (contiguous, or all with the same strides).  No two tensors may share memory, and no gradient may share it with what the step
     writes.  The scalars are fixed when the call is made, so it refuses to be captured into a HIP graph, which would replay
     the same step number."""
-    _scalars(step, lr, betas, eps, weight_decay)
-    eight = exp_avg_scales is not None
-    if eight != (exp_avg_sq_scales is not None):
-        raise ValueError("8-bit states need the scales of both")
-    scales = [exp_avg_scales, exp_avg_sq_scales] if eight else []
-    if any(len(x) != len(params) for x in [grads, exp_avgs, exp_avg_sqs] + scales):
-        raise ValueError("one gradient, two states and their scales for every parameter")
-    if not params:
-        return
-    dtype, device = params[0].dtype, params[0].device
-    if dtype not in TYPE_IDS:
-        raise TypeError("adamw_step takes float32, bfloat16 or float16 parameters, not %s" % dtype)
-    kinds = (torch.int8, torch.uint8) if eight else (torch.float32, torch.float32)
-    for what, tensors, kind in ([("a parameter", params, dtype), ("a gradient", grads, dtype), ("exp_avg", exp_avgs, kinds[0]), ("exp_avg_sq", exp_avg_sqs, kinds[1])]
-                                + [("a scale", s, torch.float32) for s in scales]):
-        if set(map(_dtype, tensors)) != {kind}:
-            raise TypeError("%s is not %s" % (what, kind))
-        if set(map(_device, tensors)) != {params[0].get_device()}:
-            raise ValueError("%s is not on %s" % (what, device))
-    shapes = list(map(_shape, params))
-    for what, tensors in (("gradient", grads), ("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
-        if list(map(_shape, tensors)) != shapes:
-            raise ValueError("the shape of a parameter and of its %s differ" % what)
-    numels = list(map(_numel, params))
-    for s in scales:
-        if list(map(_numel, s)) != list(map(_blocks, numels)) or not all(map(_contiguous, s)):
-            raise ValueError("one contiguous scale for every %d elements" % STATE_BLOCK)
-    every = [params, grads, exp_avgs, exp_avg_sqs]
-    if not all(all(map(_contiguous, x)) for x in every):
-        for p, *rest in zip(*every):
-            for what, t in zip(("a gradient", "exp_avg", "exp_avg_sq"), rest):
-                _laid_out_as(p, t, what)
-    if device.type == "cpu":
+    if isinstance(lr, torch.Tensor) or isinstance(step, torch.Tensor):
+        raise TypeError("lr and step are Python numbers")   # (reading a tensor's would wait for the GPU)
+    rc = binding().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas[0], betas[1], eps, weight_decay, exp_avg_scales, exp_avg_sq_scales)
+    check(rc)
+    if rc:   # tensors on the CPU
         with torch.no_grad():
-            for x in zip(*every, *scales):
+            for x in zip(params, grads, exp_avgs, exp_avg_sqs, *([exp_avg_scales, exp_avg_sq_scales] if exp_avg_scales is not None else [])):
                 _plain_step(*x[:4], step, lr, betas, eps, weight_decay, *x[4:])
-        return
-    if device.type != "cuda":
-        raise ValueError("adamw_step runs on the GPU or the CPU, not on %s" % device)
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("an AdamW step cannot be captured into a HIP graph: every replay would be the same step")
-    n = len(params)
-    check(library().az_adamw_step_dev(
-        device.index, current_stream(device.index), n, _pointers(params), _pointers(grads), _pointers(exp_avgs), _pointers(exp_avg_sqs),
-        _pointers(exp_avg_scales) if eight else None, _pointers(exp_avg_sq_scales) if eight else None, (C.c_int64 * n)(*numels),
-        TYPE_IDS[dtype], lr, betas[0], betas[1], eps, weight_decay, step))
-    # autograd learns that these were written, as from any operation in place: a backward pass that saved one before refuses
-    for x in [params, exp_avgs, exp_avg_sqs] + scales:
-        torch.autograd.graph.increment_version(x)
 
 
 def _plain_step(p, g, m, v, step, lr, betas, eps, weight_decay, m_scale=None, v_scale=None):
@@ -196,7 +126,8 @@ class AdamW(torch.optim.Optimizer):
     parameter is copied first."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096):
-        _scalars(1, lr, betas, eps, weight_decay)
+        if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0 and 0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError("lr, eps and weight_decay must not be negative, betas must lie in [0, 1)")
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32")
         self.state_bits, self.min_8bit_size = state_bits, int(min_8bit_size)
@@ -205,7 +136,7 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
-            if p.dtype not in TYPE_IDS:
+            if p.dtype not in TYPES:
                 raise TypeError("AdamW takes float32, bfloat16 or float16 parameters, not %s" % p.dtype)
             if not dense(p):
                 raise ValueError("AdamW needs dense parameters")

@@ -1,32 +1,33 @@
-"""What the training operators (layer_norm.py, adamw.py) share: element types, streams and errors of the C ABI."""
+"""What the training operators (layer_norm.py, adamw.py) share: the native calls behind them and the layout of tensors."""
+import importlib
+
 import torch
 
 from .. import _lib
 from ..engine import EngineError
 
-TYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # AZ_TYPE_* of include/az_engine.h
+TYPES = (torch.float32, torch.bfloat16, torch.float16)   # AZ_TYPE_* of include/az_engine.h
 
-_library = None
+_binding = None
 
 
-def library():
-    """The HIP library, for calls that take a stream of PyTorch's."""
-    global _library
-    if _library is None:
-        L = _lib.lib()
+def binding():
+    """csrc/az_torch.cpp: the training operators of the C ABI as PyTorch calls."""
+    global _binding
+    if _binding is None:
+        _lib.lib()
         # A stream belongs to the HIP runtime that made it.  _lib.lib() loads PyTorch's runtime first and the library then
         # uses the same one; a process that loaded the library by itself before that has two.
         with open("/proc/self/maps") as fh:
             runtimes = {line.split()[-1] for line in fh if "/libamdhip64.so" in line}
         if len(runtimes) > 1:
             raise RuntimeError("two HIP runtimes are loaded (%s): import torch before libazamd.so is loaded" % ", ".join(sorted(runtimes)))
-        _library = L
-    return _library
-
-
-def current_stream(device_index):
-    """Handle of PyTorch's current stream on a device."""
-    return torch._C._cuda_getCurrentRawStream(device_index)
+        try:
+            _binding = importlib.import_module("._train_ops", __package__)
+        except ImportError as e:
+            raise ImportError("alphazero_amd: network/_train_ops.so is missing or does not load (%s) - build it with "
+                              "`python -c 'import __graft_entry__ as g; g.build()'` or `make -C alphazero_amd/csrc`" % e) from e
+    return _binding
 
 
 def check(rc):

@@ -228,6 +228,13 @@ def test_norm_refuses_gradients_in_a_capture():
     assert bool(layer_norm(x, w, b).isfinite().all())       # and the process goes on
 
 
+def test_norm_refuses_a_second_derivative():
+    x, w, b, dy = _norm_case(4, 64, F32, F32, seed=18)
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(layer_norm(x, w, b), x, dy, create_graph=True)
+
+
 def test_norm_two_threads_at_once():
     import threading
     cases = [_norm_case(2000, 361, F32, F32, seed=s) for s in (20, 21)]
