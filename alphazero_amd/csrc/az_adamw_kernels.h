@@ -4,14 +4,15 @@
 //   w' = w - lr wd w - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
 // Nothing is used twice, so the step is bound by memory: 28 bytes per parameter with float32 weights and states, 16 with
-// 8-bit states (and 8 bytes of scales for every 256 parameters).
+// 8-bit states (and 16 bytes for the scales of every 256 parameters).  Measured, 24 M float32 parameters in one tensor: 112 us
+// (6.0 TB/s) and, with 8-bit state, 62 us (6.2 TB/s); a copy of 1 GiB reaches 5.1 TB/s.
 #pragma once
 #include "../../include/az_engine.h"
 #include "az_vec.h"
 
 #define AZ_ADAMW_THREADS 256
 #define AZ_ADAMW_BLOCK AZ_STATE_BLOCK    // elements that share a scale: one wave's four elements per lane
-#define AZ_ADAMW_TENSORS 56   // per launch: the table travels in the kernel's arguments, which stay under 4 KB
+#define AZ_ADAMW_TENSORS 64   // per launch: one for each lane; the table travels in the kernel's arguments, under 4 KB
 
 // The tensors of one launch.  The table goes by value: no copy to the device that would have to outlive the call, nothing
 // that a later call could overwrite while this one is still queued.
@@ -28,14 +29,13 @@ struct AdamwScalars {
     double beta1, beta2, one_minus_beta1, one_minus_beta2;
     float decay, step_size, inv_sqrt_c2, eps;   // lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
+static_assert(sizeof(AdamwTable) + sizeof(AdamwScalars) <= 4096, "kernel arguments");
 
 // Which tensor a workgroup works on: every lane compares one entry of the table (one load, where a search would be a chain).
 __device__ __forceinline__ int adamw_tensor(const AdamwTable &a, uint32_t block)
 {
-    static_assert(AZ_ADAMW_TENSORS <= 64, "one lane per tensor");
-    const int lane = threadIdx.x & 63;
-    const uint32_t last = lane < AZ_ADAMW_TENSORS ? a.last[lane] : 0xffffffffu;
-    return __popcll(__ballot(last <= block));
+    static_assert(AZ_ADAMW_TENSORS == 64, "one lane per tensor");
+    return __popcll(__ballot(a.last[threadIdx.x & 63] <= block));
 }
 
 // Square root and reciprocal by the instructions that are right to one step of float32, a third of the work of the correctly
@@ -44,13 +44,14 @@ __device__ __forceinline__ float adamw_weight(float w, float m, float v, const A
 {
     const bool small = v < 0x1p-96f;
     const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? k.inv_sqrt_c2 * 0x1p-32f : k.inv_sqrt_c2);
-    return w - k.decay * w - k.step_size * m * __builtin_amdgcn_rcpf(root + k.eps);
+    return fmaf(-k.step_size * m, __builtin_amdgcn_rcpf(root + k.eps), fmaf(-k.decay, w, w));
 }
 
+// (which products are fused is written out: a tensor's result does not depend on the form of the kernel that its size selects)
 __device__ __forceinline__ void adamw_32(float &w, float g, float &m, float &v, const AdamwScalars &k)
 {
-    m = (float)k.beta1 * m + (float)k.one_minus_beta1 * g;
-    v = (float)k.beta2 * v + (float)k.one_minus_beta2 * (g * g);
+    m = fmaf((float)k.beta1, m, (float)k.one_minus_beta1 * g);
+    v = fmaf((float)k.beta2, v, (float)k.one_minus_beta2 * (g * g));
     w = adamw_weight(w, m, v, k);
 }
 
@@ -67,19 +68,20 @@ template <int TURNS> __device__ __forceinline__ AdamwChunk adamw_chunk(const Ada
     return AdamwChunk{i, first, a.n[i] - first};
 }
 
-// FULL: the chunk ends before its tensor does, so nothing needs a check
-template <bool FULL, typename T> __device__ __forceinline__ float4 load4(const T *p, int i, int n)
+// FULL: the chunk ends before its tensor does, so nothing needs a check.  STREAM: the step's tensors together are larger
+// than every cache, so nothing of them is kept there for the next step.
+template <bool FULL, bool STREAM, typename T> __device__ __forceinline__ float4 adamw_load(const T *p, int i, int n)
 {
-    if constexpr (FULL) return load4(p + i);
+    if constexpr (FULL) return load4<STREAM>(p + i);
     else return load4(p, (int64_t)i, (int64_t)n);
 }
-template <bool FULL, typename T> __device__ __forceinline__ void store4(T *p, int i, int n, float4 f)
+template <bool FULL, bool STREAM, typename T> __device__ __forceinline__ void adamw_store(T *p, int i, int n, float4 f)
 {
-    if constexpr (FULL) store4(p + i, f);
+    if constexpr (FULL) store4<STREAM>(p + i, f);
     else store4(p, (int64_t)i, (int64_t)n, f);
 }
 
-template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adamw_32_chunk(const AdamwTable &a, const AdamwScalars &k, const AdamwChunk &c)
+template <typename T, int TURNS, bool STREAM, bool FULL> __device__ __forceinline__ void adamw_32_chunk(const AdamwTable &a, const AdamwScalars &k, const AdamwChunk &c)
 {
     T *wp = static_cast<T *>(a.param[c.tensor]) + c.first;
     const T *gp = static_cast<const T *>(a.grad[c.tensor]) + c.first;
@@ -89,7 +91,7 @@ template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adam
 #pragma unroll
     for (int u = 0; u < TURNS; u++) {
         const int at = (u * AZ_ADAMW_THREADS + threadIdx.x) * 4;
-        w[u] = load4<FULL>(wp, at, n); g[u] = load4<FULL>(gp, at, n); m[u] = load4<FULL>(mp, at, n); v[u] = load4<FULL>(vp, at, n);
+        w[u] = adamw_load<FULL, STREAM>(wp, at, n); g[u] = adamw_load<FULL, STREAM>(gp, at, n); m[u] = adamw_load<FULL, STREAM>(mp, at, n); v[u] = adamw_load<FULL, STREAM>(vp, at, n);
     }
 #pragma unroll
     for (int u = 0; u < TURNS; u++) {
@@ -98,15 +100,15 @@ template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adam
         adamw_32(w[u].y, g[u].y, m[u].y, v[u].y, k);
         adamw_32(w[u].z, g[u].z, m[u].z, v[u].z, k);
         adamw_32(w[u].w, g[u].w, m[u].w, v[u].w, k);
-        store4<FULL>(wp, at, n, w[u]); store4<FULL>(mp, at, n, m[u]); store4<FULL>(vp, at, n, v[u]);
+        adamw_store<FULL, STREAM>(wp, at, n, w[u]); adamw_store<FULL, STREAM>(mp, at, n, m[u]); adamw_store<FULL, STREAM>(vp, at, n, v[u]);
     }
 }
 
-template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_32(AdamwTable a, AdamwScalars k)
+template <typename T, int TURNS, bool STREAM> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_32(AdamwTable a, AdamwScalars k)
 {
     const AdamwChunk c = adamw_chunk<TURNS>(a);
-    if (c.left >= TURNS * 4 * AZ_ADAMW_THREADS) adamw_32_chunk<T, TURNS, true>(a, k, c);
-    else adamw_32_chunk<T, TURNS, false>(a, k, c);
+    if (c.left >= TURNS * 4 * AZ_ADAMW_THREADS) adamw_32_chunk<T, TURNS, STREAM, true>(a, k, c);
+    else adamw_32_chunk<T, TURNS, STREAM, false>(a, k, c);
 }
 
 // ---- states in 8 bits -------------------------------------------------------------------------------------------------
@@ -124,7 +126,7 @@ template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) 
 // float32 estimate of 127 sqrt(|m| / S) or 255 (v / S)^(1/4) is off by less than 1e-4 (one step each of the conversion, the
 // reciprocal, two roots and the products), so only what it puts within 2e-4 of a border, one wave in eight, is compared with
 // that border, by powers and without roots: (2c - 1)^2 S <= 254^2 |m| < (2c + 1)^2 S.  With that, 95 M bfloat16 parameters take
-// 219 us (950 MB, 4.3 TB/s); with the comparison for every element they took 360 us and were bound by arithmetic.
+// 193 us (950 MB, 4.9 TB/s); with the comparison for every element they took 360 us and were bound by arithmetic.
 // A block with an infinity or a NaN in it has a scale that is not finite and reads back as NaN as a whole.
 
 // byte e of a word as int8 / uint8, in float32: c |c| and c^2 are exact there
@@ -227,7 +229,7 @@ template <bool FULL> __device__ __forceinline__ void store_codes(uint8_t *p, int
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // A workgroup's chunk in blocks of 256, one for each of its waves at a time.
-template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adamw_8_chunk(const AdamwTable &a, const AdamwScalars &k, const AdamwChunk &ch)
+template <typename T, int TURNS, bool STREAM, bool FULL> __device__ __forceinline__ void adamw_8_chunk(const AdamwTable &a, const AdamwScalars &k, const AdamwChunk &ch)
 {
     T *wp = static_cast<T *>(a.param[ch.tensor]) + ch.first;
     const T *gp = static_cast<const T *>(a.grad[ch.tensor]) + ch.first;
@@ -242,7 +244,7 @@ template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adam
 #pragma unroll
     for (int u = 0; u < TURNS; u++) {
         const int at = (u * AZ_ADAMW_THREADS + threadIdx.x) * 4, block = u * 4 + wave;
-        w[u] = load4<FULL>(wp, at, n); g[u] = load4<FULL>(gp, at, n);
+        w[u] = adamw_load<FULL, STREAM>(wp, at, n); g[u] = adamw_load<FULL, STREAM>(gp, at, n);
         mc[u] = load_codes<FULL>(mp, at, n); vc[u] = load_codes<FULL>(vp, at, n);
         const bool in = FULL || block * AZ_ADAMW_BLOCK < n;
         ms[u] = in ? msp[block] : 0.f; vs[u] = in ? vsp[block] : 0.f;
@@ -271,7 +273,7 @@ template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adam
         // NaN has the largest magnitude bits of all, so the integer maximum keeps it
         mb = wave_umax(mb); vb = wave_umax(vb);
         const uint32_t mw = quantize_m(m, mf, mb), vw = quantize_v(v, vf, vb);
-        store4<FULL>(wp, at, n, w[u]);
+        adamw_store<FULL, STREAM>(wp, at, n, w[u]);
         store_codes<FULL>(mp, at, n, mw); store_codes<FULL>(vp, at, n, vw);
         if ((threadIdx.x & 63) == 0 && (FULL || block * AZ_ADAMW_BLOCK < n)) {
             msp[block] = __uint_as_float(mb);
@@ -280,11 +282,11 @@ template <typename T, int TURNS, bool FULL> __device__ __forceinline__ void adam
     }
 }
 
-template <typename T, int TURNS> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_8(AdamwTable a, AdamwScalars k)
+template <typename T, int TURNS, bool STREAM> __global__ __launch_bounds__(AZ_ADAMW_THREADS) void k_adamw_8(AdamwTable a, AdamwScalars k)
 {
     const AdamwChunk c = adamw_chunk<TURNS>(a);
-    if (c.left >= TURNS * 4 * AZ_ADAMW_THREADS) adamw_8_chunk<T, TURNS, true>(a, k, c);
-    else adamw_8_chunk<T, TURNS, false>(a, k, c);
+    if (c.left >= TURNS * 4 * AZ_ADAMW_THREADS) adamw_8_chunk<T, TURNS, STREAM, true>(a, k, c);
+    else adamw_8_chunk<T, TURNS, STREAM, false>(a, k, c);
 }
 
 // the values that codes stand for, rounded once to float32

@@ -26,7 +26,9 @@ hipStream_t stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStrea
 bool capturing(const at::Tensor &t)
 {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(stream_of(t), &status) != hipSuccess || status != hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream_of(t), &status) == hipSuccess) return status != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();   // (the default stream cannot be asked while another thread captures)
+    return true;
 }
 
 void launched(int rc)
@@ -128,6 +130,8 @@ std::optional<at::Tensor> layer_norm(const at::Tensor &x, const std::optional<at
     if (weight && bias && weight->scalar_type() != bias->scalar_type()) type_error("weight and bias must have one type");
     if (x.is_cpu()) return std::nullopt;
     if (!x.is_cuda()) value_error("layer_norm runs on the GPU or the CPU, not on " + x.device().str());
+    for (const at::Tensor *t : {&x, weight ? &*weight : nullptr, bias ? &*bias : nullptr})
+        if (t && t->_fw_grad(0).defined()) throw std::runtime_error("layer_norm has no forward-mode derivative on the GPU");
     const bool record = at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad()));
     py::gil_scoped_release nogil;
     if (!record) return norm_forward(x, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), eps, nullptr, nullptr);
@@ -218,11 +222,22 @@ int adamw_step(const py::sequence &params_, const py::sequence &grads_, const py
     return 0;
 }
 
-// dequantize_state of network/adamw.py, for checked tensors on the GPU
-int dequantize_state(const at::Tensor &codes, const at::Tensor &scales, const at::Tensor &out)
+// dequantize_state of network/adamw.py; nothing comes back for checked tensors on the CPU
+std::optional<at::Tensor> dequantize_state(const at::Tensor &codes, const at::Tensor &scales)
 {
-    return az_dequantize_state_dev(codes.get_device(), stream_of(codes), codes.const_data_ptr(), static_cast<const float *>(scales.const_data_ptr()), codes.numel(),
-                                   codes.scalar_type() == at::kChar, static_cast<float *>(out.data_ptr()));
+    const at::ScalarType type = codes.scalar_type();
+    if ((type != at::kChar && type != at::kByte) || scales.scalar_type() != at::kFloat)
+        type_error("a state in 8 bits is int8 or uint8 codes with float32 scales, not " + name_of(type) + " with " + name_of(scales.scalar_type()));
+    if (codes.device() != scales.device()) value_error("codes are on " + codes.device().str() + ", scales on " + scales.device().str());
+    const int64_t n = codes.numel(), blocks = (n + AZ_STATE_BLOCK - 1) / AZ_STATE_BLOCK;
+    if (!codes.is_non_overlapping_and_dense() || !scales.is_contiguous() || scales.numel() != blocks)
+        value_error(std::to_string(n) + " codes need dense memory and " + std::to_string(blocks) + " scales, not " + std::to_string(scales.numel()));
+    if (codes.is_cpu()) return std::nullopt;
+    if (!codes.is_cuda()) value_error("dequantize_state runs on the GPU or the CPU, not on " + codes.device().str());
+    at::Tensor out = at::empty_strided(codes.sizes(), codes.strides(), codes.options().dtype(at::kFloat));
+    launched(az_dequantize_state_dev(codes.get_device(), stream_of(codes), codes.const_data_ptr(), static_cast<const float *>(scales.const_data_ptr()), n,
+                                     type == at::kChar, static_cast<float *>(out.data_ptr())));
+    return out;
 }
 
 }  // namespace

@@ -153,7 +153,8 @@ int norm_sizes(int64_t rows, int64_t cols, int32_t type, int32_t affine_type, do
 {
     if (bad_type(type) || bad_type(affine_type)) return az_fail(AZ_ERR_ARG, "layer norm: unknown element type");
     if (affine_type != type && affine_type != AZ_TYPE_F32) return az_fail(AZ_ERR_ARG, "layer norm: weight and bias are float32 or of the input's type");
-    if (rows < 0 || cols < 1 || cols > ((int64_t)1 << 31) || rows > ((int64_t)1 << 40)) return az_fail(AZ_ERR_ARG, "layer norm: bad number of rows or columns");
+    // (a grid has less than 2^32 threads, of which the sums over the rows take 64 for each column)
+    if (rows < 0 || cols < 1 || cols > ((int64_t)1 << 25) || rows > ((int64_t)1 << 50) / cols) return az_fail(AZ_ERR_ARG, "layer norm: bad number of rows or columns");
     if (!(eps >= 0.0)) return az_fail(AZ_ERR_ARG, "layer norm: eps must not be negative");
     return AZ_OK;
 }
@@ -231,11 +232,12 @@ struct AdamwType {
     template <typename T> void operator()() const
     {
         if (eight) {
-            if (turns == 1) k_adamw_8<T, 1><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
-            else k_adamw_8<T, 2><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+            if (turns == 1) k_adamw_8<T, 1, false><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+            else k_adamw_8<T, 4, true><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
         } else {
-            if (turns == 1) k_adamw_32<T, 1><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
-            else k_adamw_32<T, 2><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+            if (turns == 1) k_adamw_32<T, 1, false><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+            else if (turns == 2) k_adamw_32<T, 2, false><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
+            else k_adamw_32<T, 4, true><<<blocks, AZ_ADAMW_THREADS, 0, st>>>(t, k);
         }
     }
 };
@@ -256,7 +258,7 @@ int adamw_step(int32_t device, void *stream, int64_t tensors, void *const *param
     int64_t total = 0;
     for (int64_t i = 0; i < tensors; i++) {
         const int64_t n = numels[i];
-        if (n < 0 || n > ((int64_t)1 << 40)) return az_fail(AZ_ERR_ARG, "adamw: bad tensor size");
+        if (n < 0 || n > ((int64_t)1 << 35)) return az_fail(AZ_ERR_ARG, "adamw: bad tensor size");
         if (n == 0) continue;
         if (!params[i] || !grads[i] || !m[i] || !v[i] || (eight && (!m_scales[i] || !v_scales[i]))) return az_fail(AZ_ERR_ARG, "adamw: null tensor");
         const auto add = [&](const void *p, int64_t bytes, bool written = true) { ranges.push_back(Range{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written}); };
@@ -280,15 +282,21 @@ int adamw_step(int32_t device, void *stream, int64_t tensors, void *const *param
     k.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     k.inv_sqrt_c2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
     k.eps = eps > 0.0 ? std::max((float)eps, 1.17549435e-38f) : 0.f;   // (subnormal numbers do not survive the reciprocal)
-    const int turns = total <= ((int64_t)1 << 20) ? 1 : 2;
+    // Packs of four elements to a thread, and whether the step goes past the caches.  What fits the 256 MB memory-side cache is
+    // still there at the next step (9 M float32 parameters, 252 MB: 40 us, past the caches 45); what does not only gets in its
+    // own way (24 M: 126 us through the caches, 112 past them; with 8-bit state 75 and 62).  Small steps want many workgroups
+    // (1 M: 5.4 us with one pack to a thread, 5.8 with two; 4 M: 18.2 and 17.8), steps with 8-bit state, which wait for
+    // arithmetic too, at any size (2 M: 9.0 and 9.6).
+    const int64_t bytes = total * (3 * size + (eight ? 4 : 16));
+    const int turns = bytes > ((int64_t)256 << 20) ? 4 : eight || total <= ((int64_t)1 << 20) ? 1 : 2;
     const int64_t chunk = turns * 4 * AZ_ADAMW_THREADS;
     AdamwTable t;
     int held = 0;
     uint64_t blocks = 0;
     for (int64_t i = 0; i <= tensors; i++) {
         const int64_t need = i < tensors ? (numels[i] + chunk - 1) / chunk : 0;
-        // a launch is full at 56 tensors, or when its workgroups would no longer fit the grid
-        if (held && (i == tensors || held == AZ_ADAMW_TENSORS || blocks + need > 0x40000000u)) {
+        // a launch is full at 64 tensors, or when its threads would no longer fit a grid (less than 2^32)
+        if (held && (i == tensors || held == AZ_ADAMW_TENSORS || blocks + need > 0xffffffu)) {
             for (int j = held; j < AZ_ADAMW_TENSORS; j++) t.last[j] = 0xffffffffu;
             by_type(type, AdamwType{t, k, (unsigned)blocks, eight, turns, static_cast<hipStream_t>(stream)});
             const hipError_t e = hipGetLastError();

@@ -6,21 +6,28 @@
 // Four elements of T as one load or store.  The alignment asked for is that of one element only: rows of odd length and
 // views into larger buffers start anywhere, and gfx950 takes a wide global access at any address (an unaligned one costs
 // at most one more cache line).
-template <typename T> struct Vec4 { typedef T type __attribute__((ext_vector_type(4))); };
-template <typename T> struct __attribute__((packed, aligned(alignof(T)))) Packed4 { typename Vec4<T>::type v; };
+template <typename T> struct Vec4 {
+    typedef T type __attribute__((ext_vector_type(4)));
+    typedef type any __attribute__((aligned(alignof(T))));
+};
 
-template <typename T> __device__ __forceinline__ float4 load4(const T *p)
+// STREAM: past the caches, for what will not be read again before something else has taken its place in them
+template <bool STREAM = false, typename T> __device__ __forceinline__ float4 load4(const T *p)
 {
-    const auto v = reinterpret_cast<const Packed4<T> *>(p)->v;
+    const typename Vec4<T>::any *from = reinterpret_cast<const typename Vec4<T>::any *>(p);
+    typename Vec4<T>::type v;
+    if constexpr (STREAM) v = __builtin_nontemporal_load(from);
+    else v = *from;
     return make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
 }
 
 // every conversion to 16 bits rounds to nearest even, once, from the float32 result
-template <typename T> __device__ __forceinline__ void store4(T *p, float4 f)
+template <bool STREAM = false, typename T> __device__ __forceinline__ void store4(T *p, float4 f)
 {
-    Packed4<T> out;
-    out.v = typename Vec4<T>::type{(T)f.x, (T)f.y, (T)f.z, (T)f.w};
-    *reinterpret_cast<Packed4<T> *>(p) = out;
+    const typename Vec4<T>::type v = {(T)f.x, (T)f.y, (T)f.z, (T)f.w};
+    typename Vec4<T>::any *to = reinterpret_cast<typename Vec4<T>::any *>(p);
+    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+    else *to = v;
 }
 
 // elements i .. i+3 of a run of n (those past its end are 0 / are not written)
@@ -49,7 +56,6 @@ template <typename T> struct Pack {
     typedef type any __attribute__((aligned(alignof(T))));   // at any element's address
 };
 
-// STREAM: what will not be read again from the L2 cache leaves room there for what will.
 template <bool STREAM, typename T> __device__ __forceinline__ typename Pack<T>::type load_pack(const T *p)
 {
     const typename Pack<T>::any *from = reinterpret_cast<const typename Pack<T>::any *>(p);

@@ -51,15 +51,6 @@ def quantize_state(values, signed):
     return codes, scales
 
 
-def _check_codes(codes, scales):
-    if codes.dtype not in (torch.int8, torch.uint8) or scales.dtype != torch.float32:
-        raise TypeError("a state in 8 bits is int8 or uint8 codes with float32 scales, not %s with %s" % (codes.dtype, scales.dtype))
-    if not dense(codes) or not scales.is_contiguous() or scales.numel() != _blocks(codes.numel()):
-        raise ValueError("%d codes need dense memory and %d scales, not %d" % (codes.numel(), _blocks(codes.numel()), scales.numel()))
-    if codes.device != scales.device:
-        raise ValueError("codes are on %s, scales on %s" % (codes.device, scales.device))
-
-
 def _values64(codes, scales):
     """The values of codes in memory order, in 64 bits (PyTorch)."""
     c = in_memory_order(codes).double()
@@ -69,12 +60,10 @@ def _values64(codes, scales):
 
 def dequantize_state(codes, scales):
     """The float32 values that an 8-bit state stands for, in the shape and layout of `codes`: int8 codes are m, uint8 codes v."""
-    _check_codes(codes, scales)
-    out = torch.empty_like(codes, dtype=torch.float32)
-    if codes.device.type != "cuda":
+    out = binding().dequantize_state(codes, scales)
+    if out is None:   # on the CPU
+        out = torch.empty_like(codes, dtype=torch.float32)
         in_memory_order(out).copy_(_values64(codes, scales))
-        return out
-    check(binding().dequantize_state(codes, scales, out))
     return out
 
 
@@ -123,7 +112,7 @@ class AdamW(torch.optim.Optimizer):
     8 bits (biases and other small tensors stay in 32).  A checkpoint of either kind loads into the other.
 
     Parameters are dense tensors of float32, bfloat16 or float16.  A gradient that lies in memory otherwise than its
-    parameter is copied first."""
+    parameter is copied first.  Parameters and gradients of one step may not share memory."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096):
         if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0 and 0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
@@ -185,18 +174,20 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """Takes the state of an AdamW with either kind of state and converts it to this one's."""
-        saved = state_dict["state"]
-        if any("exp_avg" not in st or "exp_avg_sq" not in st for st in saved.values()):
+        """Takes the state of an AdamW with either kind of state (PyTorch's own among them) and converts it to this one's.
+        Nothing is changed where that fails."""
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        if any("exp_avg" not in st or "exp_avg_sq" not in st for st in saved.values()) or any(k not in g for g in groups for k in self.defaults):
             raise ValueError("not the state of an AdamW optimizer")
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("the state of an optimizer with other parameter groups")
+        ids = [i for g in groups for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        new = {p: self._converted(p, saved[i]) for i, p in zip(ids, params) if i in saved}
         # PyTorch casts every state tensor to its parameter's type on loading, which codes and scales must not be: only the
         # groups go that way
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
-            if i in saved:
-                self.state[p] = self._converted(p, saved[i])
+        super().load_state_dict({"state": {}, "param_groups": groups})
+        self.state.update(new)
 
     def _converted(self, p, st):
         new = self._new_state(p)
@@ -207,7 +198,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("the state of a parameter of shape %s has shape %s" % (tuple(p.shape), tuple(old.shape)))
             scale = new.get(name + "_scale")
             if old_scale is not None and scale is not None and old.stride() == new[name].stride():
-                _check_codes(old, old_scale)
+                if old.dtype != new[name].dtype or old_scale.dtype != torch.float32 or old_scale.shape != scale.shape:
+                    raise ValueError("not the codes and scales of an 8-bit state")
                 new[name].copy_(old)
                 scale.copy_(old_scale)
                 continue

@@ -169,6 +169,23 @@ def test_norm_rows_past_32_bit_offsets():
     _check_norm(x, torch.ones(300, device=DEV), None, torch.randn(3, 300, generator=_gen(13), device=DEV).to(BF16))
 
 
+def test_norm_results_past_32_bit_offsets():
+    """More than 2^32 elements of y and dx, from one row of x and dy that is read over and over."""
+    rows, cols = (1 << 19) + 5, 8192
+    g = _gen(19)
+    x, dy = torch.randn(1, cols, generator=g, device=DEV).to(BF16), torch.randn(1, cols, generator=g, device=DEV).to(BF16)
+    w = torch.randn(cols, generator=g, device=DEV)
+    one = x.clone().requires_grad_()
+    y1 = layer_norm(one, w)
+    dx1, = torch.autograd.grad(y1, one, dy)
+    many = x.expand(rows, cols).detach().requires_grad_()
+    y = layer_norm(many, w)
+    pick = [0, 1, (1 << 18) - 1, 1 << 18, rows - 2, rows - 1]
+    assert torch.equal(y[pick], y1.expand(6, cols))
+    dx, = torch.autograd.grad(y, many, dy.expand(rows, cols))
+    assert torch.equal(dx[pick], dx1.expand(6, cols))
+
+
 def test_norm_same_bits_on_every_call():
     x, w, b, dy = _norm_case(30011, 256, F32, F32, seed=14)
     leaves = [t.requires_grad_() for t in (x, w, b)]
@@ -226,6 +243,14 @@ def test_norm_refuses_gradients_in_a_capture():
             layer_norm(x, w, b)
     torch.cuda.synchronize()
     assert bool(layer_norm(x, w, b).isfinite().all())       # and the process goes on
+
+
+def test_norm_refuses_forward_mode():
+    import torch.autograd.forward_ad as fw
+    x, w, b, dy = _norm_case(4, 64, F32, F32, seed=17)
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layer_norm(fw.make_dual(x, dy), w, b)
 
 
 def test_norm_refuses_a_second_derivative():
@@ -325,7 +350,7 @@ def test_adamw_other_constants(bits, hyper):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("count", [1, 55, 56, 57, 112, 113, 300])
+@pytest.mark.parametrize("count", [1, 55, 56, 57, 63, 64, 65, 112, 113, 128, 129, 300])
 def test_adamw_many_tensors(bits, count):
     """More tensors than one launch's table holds, of every size, empty ones among them."""
     rng = np.random.RandomState(count)
@@ -337,6 +362,37 @@ def test_adamw_many_tensors(bits, count):
 @pytest.mark.parametrize("n", [(1 << 20) - 1, (1 << 20) + 1, 5 * (1 << 20) + 257])
 def test_adamw_large_tensors(bits, n):
     _check_step(_adamw_inputs([(n,), (3,)], BF16, bits, seed=n), 3, **HYPER)
+
+
+@pytest.mark.parametrize("bits,dtype,n", [(32, F32, 9586981), (32, BF16, 12201612), (8, F32, 16777216), (8, F32, 16777217), (8, BF16, 26843546)])
+def test_adamw_steps_past_the_caches(bits, dtype, n):
+    """Around and beyond 256 MB of weights, gradients and states, from where the step streams; small tensors beside the large
+    one, so that chunks end inside a tensor."""
+    _check_step(_adamw_inputs([(5,), (n,), (4097,), (1023,)], dtype, bits, seed=n), 3, **HYPER)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_past_32_bit_offsets(bits):
+    """A tensor of more than 2^31 elements (all zeros but for three stretches), the stretches compared with the formula."""
+    n, length = (1 << 31) + 4097, 5000
+    at = [0, ((1 << 30) // 256 - 3) * 256, ((n - length) // 256) * 256]
+    small = _adamw_inputs([(length,), (length,), (n - at[2],)], BF16, bits, seed=44)
+    types = (torch.int8, torch.uint8) if bits == 8 else (F32, F32)
+    args = [[torch.zeros(n, dtype=t, device=DEV)] for t in (BF16, BF16) + types] + [[], []]
+    if bits == 8:
+        args[4], args[5] = [torch.zeros(-(-n // 256), device=DEV)], [torch.zeros(-(-n // 256), device=DEV)]
+    for k in range(6 if bits == 8 else 4):
+        for a, t in zip(at, small[k]):
+            a = a // 256 if k > 3 else a
+            args[k][0][a:a + t.numel()] = t
+    _step_all(args, 9, **HYPER)
+    _step_all(small, 9, **HYPER)      # small tensors are compared with the formula elsewhere
+    for k in range(6 if bits == 8 else 4):
+        for a, t in zip(at, small[k]):
+            a = a // 256 if k > 3 else a
+            assert torch.equal(args[k][0][a:a + t.numel()], t)
+        gap = slice((1 << 20) // (256 if k > 3 else 1), (1 << 22) // (256 if k > 3 else 1))     # between the stretches
+        assert not args[k][0][gap].any()
 
 
 @pytest.mark.parametrize("bits", [32, 8])

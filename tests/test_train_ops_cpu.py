@@ -167,10 +167,28 @@ def test_optimizer_refusals():
     sgd.step()
     with pytest.raises(ValueError, match="AdamW"):
         opt.load_state_dict(sgd.state_dict())
-    other = A.AdamW([torch.randn(10, 30, requires_grad=True)])
-    opt.step()
+    q = [torch.randn(300, requires_grad=True), torch.randn(10, 30, requires_grad=True)]
+    for t in q:
+        t.grad = torch.ones_like(t)
+    other, twin = A.AdamW(q, lr=0.5), A.AdamW([torch.randn(300, requires_grad=True), torch.randn(300, requires_grad=True)])
+    twin_p = twin.param_groups[0]["params"]
+    for t in twin_p:
+        t.grad = torch.ones_like(t)
+    other.step()
+    twin.step()
+    twin.step()
     with pytest.raises(ValueError, match="shape"):
+        other.load_state_dict(twin.state_dict())
+    assert other.param_groups[0]["lr"] == 0.5 and [other.state[t]["step"] for t in q] == [1, 1]     # nothing was changed
+    opt.step()
+    with pytest.raises(ValueError, match="groups"):
         other.load_state_dict(opt.state_dict())
+    theirs = torch.optim.AdamW(twin_p, lr=0.25)
+    theirs.step()
+    twin.load_state_dict(theirs.state_dict())        # PyTorch's own AdamW has the same state
+    assert twin.param_groups[0]["lr"] == 0.25 and twin.state[twin_p[0]]["step"] == 1
+    assert torch.equal(twin.state[twin_p[0]]["exp_avg"], theirs.state[twin_p[0]]["exp_avg"])
+    twin.step()
 
 
 @pytest.mark.parametrize("first,second", [(32, 32), (8, 8), (32, 8), (8, 32)])
@@ -229,7 +247,7 @@ def test_c_entry_points_check_their_arguments():
     err = lambda: L.az_last_error(None)  # noqa: E731
     fwd = lambda **k: L.az_layer_norm_fwd_dev(*dict(dict(device=0, stream=None, type=0, affine=0, rows=2, cols=4, eps=1e-5, x=4096, xs=4, w=None, b=None,  # noqa: E731
                                                          y=8192, ys=4, mean=None, rstd=None), **k).values())
-    for bad in (dict(type=7), dict(affine=1), dict(affine=5), dict(rows=-1), dict(cols=0), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(y=None),
+    for bad in (dict(type=7), dict(affine=1), dict(affine=5), dict(rows=-1), dict(cols=0), dict(cols=1 << 26), dict(rows=1 << 49), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(y=None),
                 dict(xs=-4), dict(ys=3), dict(mean=4096)):
         assert fwd(**bad) == _lib.ERR_ARG and b"layer norm" in err(), bad
     assert fwd(rows=0) == 0
@@ -247,7 +265,7 @@ def test_c_entry_points_check_their_arguments():
              t=1, count=2):
         return L.az_adamw_step_dev(0, None, count, ptrs(*p), ptrs(*g), ptrs(*m), ptrs(*v), ptrs(*ms) if ms else None, ptrs(*vs) if vs else None,
                                    (C.c_int64 * 2)(*n), type, lr, b1, b2, eps, wd, t)
-    for bad in (dict(count=-1), dict(type=9), dict(lr=-1.0), dict(b1=1.0), dict(b2=-0.1), dict(eps=float("nan")), dict(wd=-1.0), dict(t=0), dict(n=(-1, 10)),
+    for bad in (dict(count=-1), dict(type=9), dict(lr=-1.0), dict(b1=1.0), dict(b2=-0.1), dict(eps=float("nan")), dict(wd=-1.0), dict(t=0), dict(n=(-1, 10)), dict(n=(10, 1 << 36)),
                 dict(p=(None, 8192)), dict(g=(12288, None)), dict(ms=(36864, 40960)), dict(ms=(36864, None), vs=(45056, 49152))):
         assert step(**bad) == _lib.ERR_ARG and b"adamw" in err(), bad
     for shared in (dict(p=(4096, 4100)), dict(m=(4096, 24576)), dict(v=(20480, 32768)), dict(g=(4100, 16384)), dict(g=(20500, 16384)),
