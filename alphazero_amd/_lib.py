@@ -119,7 +119,9 @@ SIGNATURES = {
     "az_tower_flops_per_eval": (C.c_double, [_P]),
     "az_tower_conv_kernel": (C.c_char_p, [_P]),
     "az_search_run": (_I, [_P, _I]),
-    "az_layer_norm_fwd_dev": (_I, [_I, _P, _I, _I, C.c_int64, C.c_int64, C.c_double, _P, C.c_int64, _P, _P, _P, C.c_int64, _P, _P]),
+    "az_layer_norm_fwd_workspace": (C.c_int64, [_I, C.c_int64, C.c_int64]),
+    "az_layer_norm_fwd_dev": (_I, [_I, _P, _I, _I, C.c_int64, C.c_int64, C.c_double, _P, C.c_int64, _P, _P, _P, C.c_int64, _P, _P,
+                                   _P, C.c_int64]),
     "az_layer_norm_bwd_workspace": (C.c_int64, [_I, C.c_int64, C.c_int64]),
     "az_layer_norm_bwd_dev": (_I, [_I, _P, _I, _I, C.c_int64, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, _P, _P, C.c_int64,
                                    _P, _P, _P, C.c_int64]),

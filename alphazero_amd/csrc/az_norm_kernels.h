@@ -8,7 +8,7 @@
 // registers, in a second pass over those registers: a sum of squares would lose everything in rows whose mean is large
 // against their spread.
 //
-// A row belongs to TPR threads (16 or 32: part of a wave, 64: a wave, more: a workgroup), each of which holds NV packs of 16
+// A row belongs to TPR threads (4 to 32: part of a wave, 64: a wave, more: a workgroup), each of which holds NV packs of 16
 // bytes of it in registers, so a row is read from memory once; the up to 3 or 7 elements past the last whole pack are held one
 // to a thread.  Workgroups walk the rows with a stride: weights and biases
 // are loaded once per thread and not once per row, and the next row is asked for before the present one is worked on.
@@ -49,7 +49,7 @@ __device__ __forceinline__ float sum4(float4 f) { return (f.x + f.y) + (f.z + f.
 template <int TPR, int N> __device__ __forceinline__ void group_sum(float (&v)[N], float (*cell)[N][16], int slot)
 {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = TPR == 16 ? row16_sum(v[i]) : TPR == 32 ? half_sum(v[i]) : wave_sum(v[i]);
+    for (int i = 0; i < N; i++) v[i] = TPR == 4 ? quad_sum(v[i]) : TPR == 8 ? oct_sum(v[i]) : TPR == 16 ? row16_sum(v[i]) : TPR == 32 ? half_sum(v[i]) : wave_sum(v[i]);
     if constexpr (TPR > 64) {
         constexpr int WAVES = TPR / 64;
         const int wave = threadIdx.x >> 6;
@@ -211,6 +211,70 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
     }
 }
 
+// A few rows that are too wide: a workgroup to a chunk of 8192 elements, in two launches.  The first leaves each chunk's mean
+// and its sum of squared distances from that mean; the second puts them together,
+//   mean = sum n_i mean_i / n,   sum of squares = sum (M2_i + n_i (mean_i - mean)^2),
+// and writes its chunk.  3 rows of 300 k float32: 18 us, with a workgroup to each row 72.
+#define AZ_NORM_CHUNK 8192
+
+// the elements of thread threadIdx.x's pack k of four in the chunk
+__device__ __forceinline__ int64_t chunk_at(int k) { return (int64_t)blockIdx.x * AZ_NORM_CHUNK + (k * AZ_NORM_WIDE_THREADS + threadIdx.x) * 4; }
+
+template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_layer_norm_chunk_stats(NormFwd a, float2 *part)
+{
+    __shared__ float cell[AZ_NORM_WIDE_THREADS / 64];
+    constexpr int NV = AZ_NORM_CHUNK / (AZ_NORM_WIDE_THREADS * 4);
+    const T *x = static_cast<const T *>(a.x) + blockIdx.y * a.x_stride;
+    const float n = (float)min((int64_t)AZ_NORM_CHUNK, a.cols - (int64_t)blockIdx.x * AZ_NORM_CHUNK);
+    float4 v[NV];
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; k++) { v[k] = load4(x, chunk_at(k), a.cols); s += sum4(v[k]); }
+    const float mean = mean_of(block_sum(s, cell), n, 1.0f / n);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int64_t c = chunk_at(k);
+        const float d0 = v[k].x - mean, d1 = v[k].y - mean, d2 = v[k].z - mean, d3 = v[k].w - mean;
+        if (c < a.cols) q += d0 * d0;
+        if (c + 1 < a.cols) q += d1 * d1;
+        if (c + 2 < a.cols) q += d2 * d2;
+        if (c + 3 < a.cols) q += d3 * d3;
+    }
+    q = block_sum(q, cell);
+    if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = make_float2(mean, q);
+}
+
+template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_layer_norm_chunk_write(NormFwd a, const float2 *part)
+{
+    __shared__ float cell[AZ_NORM_WIDE_THREADS / 64];
+    constexpr int NV = AZ_NORM_CHUNK / (AZ_NORM_WIDE_THREADS * 4);
+    const T *x = static_cast<const T *>(a.x) + blockIdx.y * a.x_stride;
+    T *y = static_cast<T *>(a.y) + blockIdx.y * a.y_stride;
+    float4 v[NV], w[NV], b[NV];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        v[k] = load4(x, chunk_at(k), a.cols);
+        w[k] = load_affine<T>(a.w, a.affine_f32, chunk_at(k), a.cols, 1.0f);
+        b[k] = load_affine<T>(a.b, a.affine_f32, chunk_at(k), a.cols, 0.0f);
+    }
+    part += (int64_t)blockIdx.y * gridDim.x;
+    const float n = (float)a.cols, inv = 1.0f / n;
+    const auto count = [&](unsigned i) { return (float)min((int64_t)AZ_NORM_CHUNK, a.cols - (int64_t)i * AZ_NORM_CHUNK); };
+    float s = 0.f, q = 0.f;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += AZ_NORM_WIDE_THREADS) s += count(i) * part[i].x;
+    const float mean = mean_of(block_sum(s, cell), n, inv);
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += AZ_NORM_WIDE_THREADS) {
+        const float d = part[i].x - mean;
+        q += part[i].y + count(i) * d * d;
+    }
+    const float r = inv_sqrt(block_sum(q, cell) * inv + a.eps);
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        store4(y, chunk_at(k), a.cols, make_float4((v[k].x - mean) * r * w[k].x + b[k].x, (v[k].y - mean) * r * w[k].y + b[k].y,
+                                                   (v[k].z - mean) * r * w[k].z + b[k].z, (v[k].w - mean) * r * w[k].w + b[k].w));
+    if (a.mean && blockIdx.x == 0 && threadIdx.x == 0) { a.mean[blockIdx.y] = mean; a.rstd[blockIdx.y] = r; }
+}
+
 struct NormBwd {
     const void *dy, *x, *w;
     const float *mean, *rstd;
@@ -362,6 +426,50 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
                    make_float4(r * (g.x * w.x - m0 - (v.x - mean) * r * m1), r * (g.y * w.y - m0 - (v.y - mean) * r * m1),
                                r * (g.z * w.z - m0 - (v.z - mean) * r * m1), r * (g.w * w.w - m0 - (v.w - mean) * r * m1)));
         }
+    }
+}
+
+// The same for a few rows, in chunks as forward: the chunks' two sums, then dx.
+template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_layer_norm_chunk_sums(NormBwd a, float2 *part)
+{
+    __shared__ float cell[AZ_NORM_WIDE_THREADS / 64];
+    constexpr int NV = AZ_NORM_CHUNK / (AZ_NORM_WIDE_THREADS * 4);
+    const T *x = static_cast<const T *>(a.x) + blockIdx.y * a.x_stride, *dy = static_cast<const T *>(a.dy) + blockIdx.y * a.dy_stride;
+    const float mean = a.mean[blockIdx.y], r = a.rstd[blockIdx.y];
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int64_t c = chunk_at(k);
+        const float4 v = load4(x, c, a.cols), g = load4(dy, c, a.cols), w = load_affine<T>(a.w, a.affine_f32, c, a.cols, 1.0f);
+        const float g0 = g.x * w.x, g1 = g.y * w.y, g2 = g.z * w.z, g3 = g.w * w.w;
+        if (c < a.cols) { s0 += g0; s1 += g0 * ((v.x - mean) * r); }
+        if (c + 1 < a.cols) { s0 += g1; s1 += g1 * ((v.y - mean) * r); }
+        if (c + 2 < a.cols) { s0 += g2; s1 += g2 * ((v.z - mean) * r); }
+        if (c + 3 < a.cols) { s0 += g3; s1 += g3 * ((v.w - mean) * r); }
+    }
+    s0 = block_sum(s0, cell);
+    s1 = block_sum(s1, cell);
+    if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = make_float2(s0, s1);
+}
+
+template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_layer_norm_chunk_dx(NormBwd a, const float2 *part)
+{
+    __shared__ float cell[AZ_NORM_WIDE_THREADS / 64];
+    constexpr int NV = AZ_NORM_CHUNK / (AZ_NORM_WIDE_THREADS * 4);
+    const T *x = static_cast<const T *>(a.x) + blockIdx.y * a.x_stride, *dy = static_cast<const T *>(a.dy) + blockIdx.y * a.dy_stride;
+    T *dx = static_cast<T *>(a.dx) + blockIdx.y * a.dx_stride;
+    const float mean = a.mean[blockIdx.y], r = a.rstd[blockIdx.y], inv = 1.0f / (float)a.cols;
+    part += (int64_t)blockIdx.y * gridDim.x;
+    float s0 = 0.f, s1 = 0.f;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += AZ_NORM_WIDE_THREADS) { s0 += part[i].x; s1 += part[i].y; }
+    const float m0 = block_sum(s0, cell) * inv, m1 = block_sum(s1, cell) * inv;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int64_t c = chunk_at(k);
+        const float4 v = load4(x, c, a.cols), g = load4(dy, c, a.cols), w = load_affine<T>(a.w, a.affine_f32, c, a.cols, 1.0f);
+        store4(dx, c, a.cols,
+               make_float4(r * (g.x * w.x - m0 - (v.x - mean) * r * m1), r * (g.y * w.y - m0 - (v.y - mean) * r * m1),
+                           r * (g.z * w.z - m0 - (v.z - mean) * r * m1), r * (g.w * w.w - m0 - (v.w - mean) * r * m1)));
     }
 }
 

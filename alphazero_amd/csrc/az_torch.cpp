@@ -63,9 +63,12 @@ at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &weight, const at:
     const auto [v, stride] = as_rows(x, cols);
     const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
     const at::ScalarType affine = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
-    at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    launched(az_layer_norm_fwd_dev(x.get_device(), stream_of(x), type_id(x.scalar_type()), type_id(affine), rows, cols, eps, v.const_data_ptr(), stride,
-                                   pointer(w), pointer(b), y.data_ptr(), cols, mean, rstd));
+    const int32_t type = type_id(x.scalar_type());
+    at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), space;
+    const int64_t n = az_layer_norm_fwd_workspace(type, rows, cols);
+    if (n) space = at::empty({n}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+    launched(az_layer_norm_fwd_dev(x.get_device(), stream_of(x), type, type_id(affine), rows, cols, eps, v.const_data_ptr(), stride,
+                                   pointer(w), pointer(b), y.data_ptr(), cols, mean, rstd, n ? static_cast<float *>(space.data_ptr()) : nullptr, n));
     return y;
 }
 
@@ -101,7 +104,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), options);
         if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty({cols}, options.dtype(affine));
         if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = at::empty({cols}, options.dtype(affine));
-        const int64_t n = dw.defined() || db.defined() ? az_layer_norm_bwd_workspace(type, rows, cols) : 0;
+        const int64_t n = az_layer_norm_bwd_workspace(type, rows, cols);
         if (n) space = at::empty({n}, options.dtype(at::kFloat));
         const float *at = static_cast<const float *>(stats.const_data_ptr());
         launched(az_layer_norm_bwd_dev(x.get_device(), stream_of(x), type, type_id(affine), rows, cols, g.const_data_ptr(), dy_stride, v.const_data_ptr(), x_stride,

@@ -79,8 +79,23 @@ template <int CTRL> __device__ __forceinline__ uint32_t dpp_row(uint32_t x)
 }
 #define AZ_ROW_ROR(n) (0x120 + (n))   // DPP row_ror: rotation within 16 lanes
 
-// Sum over the 16 lanes of a DPP row, in every lane, the same bits in all of them (each step adds the same two partial
+#define AZ_QUAD_XOR1 0xb1               // DPP quad_perm 1,0,3,2
+#define AZ_QUAD_XOR2 0x4e               // DPP quad_perm 2,3,0,1
+#define AZ_ROW_HALF_MIRROR 0x141        // DPP row_half_mirror: lane i of eight takes lane 7 - i
+
+// Sums over 4 and 8 neighbouring lanes and over the 16 lanes of a DPP row, in every lane, the same bits in all of them (each step adds the same two partial
 // sums in both of the lanes that hold them).
+__device__ __forceinline__ float quad_sum(float x)
+{
+    x += __uint_as_float(dpp_row<AZ_QUAD_XOR1>(__float_as_uint(x)));
+    x += __uint_as_float(dpp_row<AZ_QUAD_XOR2>(__float_as_uint(x)));
+    return x;
+}
+__device__ __forceinline__ float oct_sum(float x)
+{
+    x = quad_sum(x);
+    return x + __uint_as_float(dpp_row<AZ_ROW_HALF_MIRROR>(__float_as_uint(x)));
+}
 __device__ __forceinline__ float row16_sum(float x)
 {
     x += __uint_as_float(dpp_row<AZ_ROW_ROR(8)>(__float_as_uint(x)));

@@ -341,13 +341,15 @@ int az_tower_leaf_compaction(az_engine *h, int32_t on);
 #define AZ_TYPE_F16 2
 /* Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias for `rows` rows of `cols` elements; row i of x
  * starts at element i * x_stride (0: the same row throughout).  weight / bias may be NULL (1 / 0) and are of affine_type, float32 or
- * x's type.  mean / rstd (float32, [rows]): what the backward pass needs, or both NULL. */
+ * x's type.  mean / rstd (float32, [rows]): what the backward pass needs, or both NULL.  workspace: 8-byte aligned,
+ * az_layer_norm_fwd_workspace(type, rows, cols) floats (0 but for a few very wide rows); a workspace may be reused as soon as the
+ * stream has passed the call. */
+int64_t az_layer_norm_fwd_workspace(int32_t type, int64_t rows, int64_t cols);
 int az_layer_norm_fwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, double eps,
                           const void *x, int64_t x_stride, const void *weight, const void *bias, void *y, int64_t y_stride,
-                          float *mean, float *rstd);
+                          float *mean, float *rstd, float *workspace, int64_t workspace_floats);
 /* Its gradient: dx (of x's type), dweight and dbias (of affine_type, sums over the rows, the same bits on every call); each may
- * be NULL if not wanted.  workspace: az_layer_norm_bwd_workspace(type, rows, cols) floats, needed for dweight / dbias; it may be reused
- * as soon as the stream has passed the call. */
+ * be NULL if not wanted.  workspace: 8-byte aligned, az_layer_norm_bwd_workspace(type, rows, cols) floats. */
 int64_t az_layer_norm_bwd_workspace(int32_t type, int64_t rows, int64_t cols);
 int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, const void *dy,
                           int64_t dy_stride, const void *x, int64_t x_stride, const void *weight, const float *mean, const float *rstd,

@@ -73,6 +73,20 @@ def test_norm_every_number_of_rows(rows, cols, dtype, affine):
     _check_norm(*_norm_case(rows, cols, dtype, affine, seed=rows))
 
 
+@pytest.mark.parametrize("rows,cols", [(3, 8193), (255, 8200), (256, 8200), (257, 12345), (3, 300000), (1, 1000001), (100, 24576), (2, 16384), (2, 16385)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm_wide_rows_in_chunks(rows, cols, dtype):
+    """Rows too wide for a workgroup, few of them (in chunks) and many."""
+    _check_norm(*_norm_case(rows, cols, dtype, F32, seed=rows))
+
+
+@pytest.mark.parametrize("cols", range(1, 41))
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm_narrow_rows(cols, dtype):
+    for rows in (1, 63, 64, 65, 5000):
+        _check_norm(*_norm_case(rows, cols, dtype, F32, seed=cols))
+
+
 @pytest.mark.parametrize("cols", [20, 256, 3000, 9000])
 @pytest.mark.parametrize("weight,bias", [(False, False), (True, False), (False, True)])
 def test_norm_without_weight_or_bias(cols, weight, bias):

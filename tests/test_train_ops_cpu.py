@@ -246,15 +246,19 @@ def test_c_entry_points_check_their_arguments():
     L = _lib.lib()
     err = lambda: L.az_last_error(None)  # noqa: E731
     fwd = lambda **k: L.az_layer_norm_fwd_dev(*dict(dict(device=0, stream=None, type=0, affine=0, rows=2, cols=4, eps=1e-5, x=4096, xs=4, w=None, b=None,  # noqa: E731
-                                                         y=8192, ys=4, mean=None, rstd=None), **k).values())
+                                                         y=8192, ys=4, mean=None, rstd=None, space=None, n=0), **k).values())
     for bad in (dict(type=7), dict(affine=1), dict(affine=5), dict(rows=-1), dict(cols=0), dict(cols=1 << 26), dict(rows=1 << 49), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(y=None),
                 dict(xs=-4), dict(ys=3), dict(mean=4096)):
         assert fwd(**bad) == _lib.ERR_ARG and b"layer norm" in err(), bad
     assert fwd(rows=0) == 0
+    assert L.az_layer_norm_fwd_workspace(0, 2, 8192) == 0 and L.az_layer_norm_fwd_workspace(0, 300, 100000) == 0
+    assert L.az_layer_norm_fwd_workspace(0, 3, 20000) == 18 and L.az_layer_norm_fwd_workspace(9, 3, 20000) == 0
+    for bad in (dict(n=17), dict(space=4100), dict(space=None)):
+        assert fwd(**dict(dict(rows=3, cols=20000, xs=20000, ys=20000, space=4096, n=18), **bad)) == _lib.ERR_ARG and b"workspace" in err()
     bwd = lambda **k: L.az_layer_norm_bwd_dev(*dict(dict(device=0, stream=None, type=0, affine=0, rows=2, cols=4, dy=4096, dys=4, x=4096, xs=4, w=None, mean=4096,  # noqa: E731
                                                          rstd=4096, dx=8192, dxs=4, dw=4096, db=None, space=4096, n=16), **k).values())
     assert L.az_layer_norm_bwd_workspace(0, 2, 4) == 8 and not any(L.az_layer_norm_bwd_workspace(*x) for x in ((0, 0, 4), (0, -1, 4), (9, 2, 4)))
-    for bad in (dict(type=3), dict(dy=None), dict(x=None), dict(mean=None), dict(n=7), dict(space=None), dict(dxs=3), dict(dys=-1)):
+    for bad in (dict(type=3), dict(dy=None), dict(x=None), dict(mean=None), dict(n=7), dict(space=None), dict(space=4100), dict(dxs=3), dict(dys=-1)):
         assert bwd(**bad) == _lib.ERR_ARG and b"layer norm" in err(), bad
     assert bwd(dx=None, dw=None) == 0
 
