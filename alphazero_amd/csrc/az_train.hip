@@ -292,7 +292,7 @@ int adamw_step(int32_t device, void *stream, int64_t tensors, void *const *param
     int64_t total = 0;
     for (int64_t i = 0; i < tensors; i++) {
         const int64_t n = numels[i];
-        if (n < 0 || n > ((int64_t)1 << 35)) return az_fail(AZ_ERR_ARG, "adamw: bad tensor size");
+        if (n < 0 || n > ((int64_t)1 << 33)) return az_fail(AZ_ERR_ARG, "adamw: bad tensor size");
         if (n == 0) continue;
         if (!params[i] || !grads[i] || !m[i] || !v[i] || (eight && (!m_scales[i] || !v_scales[i]))) return az_fail(AZ_ERR_ARG, "adamw: null tensor");
         const auto add = [&](const void *p, int64_t bytes, bool written = true) { ranges.push_back(Range{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written}); };
@@ -316,34 +316,35 @@ int adamw_step(int32_t device, void *stream, int64_t tensors, void *const *param
     k.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     k.inv_sqrt_c2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
     k.eps = eps > 0.0 ? std::max((float)eps, 1.17549435e-38f) : 0.f;   // (subnormal numbers do not survive the reciprocal)
-    // Packs of four elements to a thread, and whether the step goes past the caches.  What fits the 256 MB memory-side cache is
-    // still there at the next step (9 M float32 parameters, 252 MB: 40 us, past the caches 45); what does not only gets in its
-    // own way (24 M: 126 us through the caches, 112 past them; with 8-bit state 75 and 62).  Small steps want many workgroups
-    // (1 M: 5.4 us with one pack to a thread, 5.8 with two; 4 M: 18.2 and 17.8), steps with 8-bit state, which wait for
-    // arithmetic too, at any size (2 M: 9.0 and 9.6).
-    const int64_t bytes = total * (3 * size + (eight ? 4 : 16));
-    const int turns = bytes > ((int64_t)256 << 20) ? 4 : eight || total <= ((int64_t)1 << 20) ? 1 : 2;
-    const int64_t chunk = turns * 4 * AZ_ADAMW_THREADS;
+    // What fits the 256 MB memory-side cache is still there at the next step (9 M float32 parameters, 252 MB: 40 us, past the
+    // caches 45); what does not only gets in its own way (24 M: 126 us through the caches, 112 past them; with 8-bit state 75
+    // and 62).
+    const bool stream_past = total * (3 * size + (eight ? 4 : 16)) > ((int64_t)256 << 20);
     AdamwTable t;
-    int held = 0;
-    uint64_t blocks = 0;
-    for (int64_t i = 0; i <= tensors; i++) {
-        const int64_t need = i < tensors ? (numels[i] + chunk - 1) / chunk : 0;
+    for (int64_t i = 0; i < tensors;) {
         // a launch is full at 64 tensors, or when its threads would no longer fit a grid (less than 2^32)
-        if (held && (i == tensors || held == AZ_ADAMW_TENSORS || blocks + need > 0xffffffu)) {
-            for (int j = held; j < AZ_ADAMW_TENSORS; j++) t.last[j] = 0xffffffffu;
-            by_type(type, AdamwType{t, k, (unsigned)blocks, eight, turns, static_cast<hipStream_t>(stream)});
-            const hipError_t e = hipGetLastError();
-            if (e != hipSuccess) return fail_hip("adamw", e);
-            held = 0;
-            blocks = 0;
+        int held = 0;
+        int64_t elements = 0, widest = 0;
+        for (; i < tensors && held < AZ_ADAMW_TENSORS; i++) {
+            const int64_t n = numels[i];
+            if (n == 0) continue;
+            if (held && widest + n / 1024 + 1 > 0xffffff) break;
+            widest += n / 1024 + 1;
+            elements += n;
+            t.param[held] = params[i]; t.grad[held] = grads[i]; t.m[held] = m[i]; t.v[held] = v[i];
+            t.m_scale[held] = eight ? m_scales[i] : nullptr; t.v_scale[held] = eight ? v_scales[i] : nullptr;
+            t.n[held++] = n;
         }
-        if (i == tensors || need == 0) continue;
-        blocks += need;
-        t.param[held] = params[i]; t.grad[held] = grads[i]; t.m[held] = m[i]; t.v[held] = v[i];
-        t.m_scale[held] = eight ? m_scales[i] : nullptr; t.v_scale[held] = eight ? v_scales[i] : nullptr;
-        t.n[held] = numels[i];
-        t.last[held++] = (uint32_t)blocks;
+        if (!held) break;
+        // Packs of four elements to a thread.  Small launches want many workgroups (1 M: 5.4 us with one pack, 5.8 with two; 4 M:
+        // 18.2 and 17.8), launches with 8-bit state, which wait for arithmetic too, at any size (2 M: 9.0 and 9.6).
+        const int turns = elements <= ((int64_t)1 << 20) ? 1 : stream_past ? 4 : eight ? 1 : 2;
+        const int64_t chunk = turns * 4 * AZ_ADAMW_THREADS;
+        uint32_t blocks = 0;
+        for (int j = 0; j < AZ_ADAMW_TENSORS; j++) t.last[j] = j < held ? blocks += (uint32_t)((t.n[j] + chunk - 1) / chunk) : 0xffffffffu;
+        by_type(type, AdamwType{t, k, blocks, eight, turns, static_cast<hipStream_t>(stream)});
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return fail_hip("adamw", e);
     }
     return AZ_OK;
 }
