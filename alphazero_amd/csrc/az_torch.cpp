@@ -104,7 +104,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), options);
         if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty({cols}, options.dtype(affine));
         if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = at::empty({cols}, options.dtype(affine));
-        const int64_t n = az_layer_norm_bwd_workspace(type, rows, cols);
+        const int64_t n = dw.defined() || db.defined() ? az_layer_norm_bwd_workspace(type, rows, cols) : az_layer_norm_fwd_workspace(type, rows, cols);
         if (n) space = at::empty({n}, options.dtype(at::kFloat));
         const float *at = static_cast<const float *>(stats.const_data_ptr());
         launched(az_layer_norm_bwd_dev(x.get_device(), stream_of(x), type, type_id(affine), rows, cols, g.const_data_ptr(), dy_stride, v.const_data_ptr(), x_stride,

@@ -226,9 +226,9 @@ extern "C" int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type,
     if (rows > 0 && (!dy || !x || !mean || !rstd)) return az_fail(AZ_ERR_ARG, "layer norm backward: null array");
     if (dy_stride < 0 || x_stride < 0 || (dx && dx_stride < cols && rows > 1)) return az_fail(AZ_ERR_ARG, "layer norm backward: bad row stride");
     const bool sums = dweight || dbias;
-    const int64_t need = az_layer_norm_bwd_workspace(type, rows, cols);
     const int64_t chunk_floats = 2 * rows * norm_chunks(rows, cols, type);   // first in the workspace: pairs, so its start is aligned
-    if ((sums || (dx && chunk_floats)) && need > 0 && (!workspace || workspace_floats < need || (uintptr_t)workspace % 8)) return az_fail(AZ_ERR_ARG, "layer norm backward: workspace smaller than az_layer_norm_bwd_workspace, or not aligned to 8 bytes");
+    const int64_t need = sums ? az_layer_norm_bwd_workspace(type, rows, cols) : dx ? chunk_floats : 0;
+    if (need > 0 && (!workspace || workspace_floats < need || (uintptr_t)workspace % 8)) return az_fail(AZ_ERR_ARG, "layer norm backward: workspace smaller than az_layer_norm_bwd_workspace, or not aligned to 8 bytes");
     if (!dx && !sums) return AZ_OK;
     DeviceScope scope(device);
     if (scope.error != hipSuccess) return fail_hip("layer norm backward: device", scope.error);

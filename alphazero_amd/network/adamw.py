@@ -122,13 +122,20 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.min_8bit_size = state_bits, int(min_8bit_size)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):   # (what copy and pickle take along)
+        return dict(super().__getstate__(), state_bits=self.state_bits, min_8bit_size=self.min_8bit_size)
+
     def add_param_group(self, group):
         super().add_param_group(group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dtype not in TYPES:
-                raise TypeError("AdamW takes float32, bfloat16 or float16 parameters, not %s" % p.dtype)
-            if not dense(p):
-                raise ValueError("AdamW needs dense parameters")
+        try:
+            for p in self.param_groups[-1]["params"]:
+                if p.dtype not in TYPES:
+                    raise TypeError("AdamW takes float32, bfloat16 or float16 parameters, not %s" % p.dtype)
+                if not dense(p):
+                    raise ValueError("AdamW needs dense parameters")
+        except Exception:
+            self.param_groups.pop()
+            raise
 
     def _eight(self, p):
         return self.state_bits == 8 and p.numel() >= self.min_8bit_size
@@ -142,6 +149,9 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            # (before a state is made, whose memory would be the graph's)
+            raise RuntimeError("an AdamW step cannot be captured into a HIP graph: every replay would be the same step")
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -335,7 +335,8 @@ int az_tower_leaf_compaction(az_engine *h, int32_t on);
  * and products.  No counterpart in the reference, which has batch norm and momentum SGD only.  These calls need no engine:
  * `device` is the HIP device of the arrays and `stream` a stream of that device (NULL: its default stream), on which the work is
  * queued - they return without waiting.  All arrays are device memory, element types are AZ_TYPE_*.  The calling thread's
- * current device is left as it was.  Any number of threads may call at once.  az_last_error(NULL) says why a call failed. */
+ * current device is left as it was.  Any number of threads may call at once.  What a call writes may not overlap what it reads,
+ * but for AdamW's tensors, which are updated in place.  az_last_error(NULL) says why a call failed. */
 #define AZ_TYPE_F32 0
 #define AZ_TYPE_BF16 1
 #define AZ_TYPE_F16 2
@@ -349,7 +350,8 @@ int az_layer_norm_fwd_dev(int32_t device, void *stream, int32_t type, int32_t af
                           const void *x, int64_t x_stride, const void *weight, const void *bias, void *y, int64_t y_stride,
                           float *mean, float *rstd, float *workspace, int64_t workspace_floats);
 /* Its gradient: dx (of x's type), dweight and dbias (of affine_type, sums over the rows, the same bits on every call); each may
- * be NULL if not wanted.  workspace: 8-byte aligned, az_layer_norm_bwd_workspace(type, rows, cols) floats. */
+ * be NULL if not wanted.  workspace: 8-byte aligned, az_layer_norm_bwd_workspace(type, rows, cols) floats; for dx alone as many as
+ * forward. */
 int64_t az_layer_norm_bwd_workspace(int32_t type, int64_t rows, int64_t cols);
 int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type, int32_t affine_type, int64_t rows, int64_t cols, const void *dy,
                           int64_t dy_stride, const void *x, int64_t x_stride, const void *weight, const float *mean, const float *rstd,

@@ -228,8 +228,9 @@ def test_norm_gradient_against_differences():
             assert abs((ends[0] - ends[1]) / (2 * e) - float(g.view(-1)[i])) < 5e-3
 
 
-def test_norm_other_stream_and_capture():
-    x, w, b, dy = _norm_case(512, 722, F32, F32, seed=16)
+@pytest.mark.parametrize("rows,cols", [(512, 722), (3, 20000), (300, 9000)])
+def test_norm_other_stream_and_capture(rows, cols):
+    x, w, b, dy = _norm_case(rows, cols, F32, F32, seed=16)
     want = layer_norm(x, w, b)
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
@@ -241,7 +242,7 @@ def test_norm_other_stream_and_capture():
     with torch.cuda.graph(graph):
         held = layer_norm(x, w, b)
     for seed in (1, 2, 3):                       # replays see the new input, eager work in between
-        x.copy_(_norm_case(512, 722, F32, F32, seed=seed)[0])
+        x.copy_(_norm_case(rows, cols, F32, F32, seed=seed)[0])
         eager = layer_norm(x, w, b)
         graph.replay()
         torch.cuda.synchronize()
@@ -504,6 +505,24 @@ def test_adamw_refusals():
     A.adamw_step(p, [g[0], g[0][:50]], m, v, 1)           # two gradients may be the same memory
     with pytest.raises(ValueError, match="not on"):
         A.adamw_step(p, [g[0], g[1].cpu()], m, v, 1)
+
+
+def test_adamw_refused_capture_leaves_no_state():
+    """A first step that is refused in a capture has made no state in the graph's memory; the next one is right."""
+    w = [torch.randn(5000, generator=_gen(k), device=DEV).requires_grad_() for k in (1, 1)]
+    a, b = A.AdamW(w[:1], state_bits=8), A.AdamW(w[1:], state_bits=8)
+    for t in w:
+        t.grad = torch.randn(5000, generator=_gen(2), device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            a.step()
+    torch.cuda.synchronize()
+    assert not a.state
+    del graph
+    a.step()
+    b.step()
+    assert torch.equal(w[0].detach(), w[1].detach())
 
 
 def test_adamw_tells_autograd():

@@ -162,6 +162,9 @@ def test_optimizer_refusals():
     with pytest.raises(ValueError):
         A.AdamW([torch.nn.Parameter(torch.randn(6)[::2])])
     opt = A.AdamW([p])
+    with pytest.raises(TypeError):
+        opt.add_param_group({"params": [torch.randn(3, dtype=torch.float64, requires_grad=True)]})
+    assert len(opt.param_groups) == 1
     sgd = torch.optim.SGD([p], lr=0.1, momentum=0.9)
     p.grad = torch.ones_like(p)
     sgd.step()
@@ -189,6 +192,25 @@ def test_optimizer_refusals():
     assert twin.param_groups[0]["lr"] == 0.25 and twin.state[twin_p[0]]["step"] == 1
     assert torch.equal(twin.state[twin_p[0]]["exp_avg"], theirs.state[twin_p[0]]["exp_avg"])
     twin.step()
+
+
+def test_optimizer_copies():
+    import copy
+    import pickle
+    torch.manual_seed(6)
+    p = torch.randn(5000, requires_grad=True)
+    opt = A.AdamW([p], state_bits=8, min_8bit_size=100)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.state_bits == 8 and other.min_8bit_size == 100
+        q, = other.param_groups[0]["params"]
+        q.grad = p.grad.clone()
+        other.step()
+        assert other.state[q]["step"] == 2 and "exp_avg_scale" in other.state[q]
+        last = q.detach().clone()
+    opt.step()
+    assert torch.equal(p.detach(), last)
 
 
 @pytest.mark.parametrize("first,second", [(32, 32), (8, 8), (32, 8), (8, 32)])
