@@ -125,7 +125,8 @@ template <typename T, int TURNS, bool STREAM> __global__ __launch_bounds__(AZ_AD
 // Codes are those of the 64-bit means too: a value next to a border between two codes goes to the right side of it.  A
 // float32 estimate of 127 sqrt(|m| / S) or 255 (v / S)^(1/4) is off by less than 1e-4 (one step each of the conversion, the
 // reciprocal, two roots and the products), so only what it puts within 2e-4 of a border, one wave in eight, is compared with
-// that border, by powers and without roots: (2c - 1)^2 S <= 254^2 |m| < (2c + 1)^2 S.  With that, 95 M bfloat16 parameters take
+// that border, by powers and without roots: (2c - 1)^2 S < 254^2 |m| < (2c + 1)^2 S.  A value on a border goes to the even code
+// (with b2 = 0 and 16-bit gradients that happens: both sides of the comparison round the same product then, and are equal).  With that, 95 M bfloat16 parameters take
 // 193 us (950 MB, 4.9 TB/s); with the comparison for every element they took 360 us and were bound by arithmetic.
 // A block with an infinity or a NaN in it has a scale that is not finite and reads back as NaN as a whole.
 
@@ -147,7 +148,8 @@ __device__ __forceinline__ float border_m(double m, double s, double inv)
     const double a = fabs(m), t = a * 64516.0;   // 254^2
     const int c = (int)rintf(127.0f * __builtin_amdgcn_sqrtf((float)(a * inv)));
     const double lo = (double)((2 * c - 1) * abs(2 * c - 1)) * s, hi = (double)((2 * c + 1) * (2 * c + 1)) * s;
-    return (float)min(c + (t >= hi ? 1 : 0) - (t < lo ? 1 : 0), 127);
+    const bool odd = c & 1;
+    return (float)min(c + (t > hi || (t == hi && odd) ? 1 : 0) - (t < lo || (t == lo && odd) ? 1 : 0), 127);
 }
 
 __device__ __forceinline__ float border_v(double v, double s, double inv)
@@ -155,7 +157,9 @@ __device__ __forceinline__ float border_v(double v, double s, double inv)
     const double t = v * 67652010000.0;          // 510^4
     const int c = (int)rintf(255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)(v * inv))));
     const double l = (double)((2 * c - 1) * abs(2 * c - 1)), h = (double)((2 * c + 1) * (2 * c + 1));
-    return (float)min(c + (t >= h * h * s ? 1 : 0) - (t < l * fabs(l) * s ? 1 : 0), 255);
+    const double lo = l * fabs(l) * s, hi = h * h * s;
+    const bool odd = c & 1;
+    return (float)min(c + (t > hi || (t == hi && odd) ? 1 : 0) - (t < lo || (t == lo && odd) ? 1 : 0), 255);
 }
 
 // four codes as the bytes of a word; `bits` are the scale's, the same in the whole wave

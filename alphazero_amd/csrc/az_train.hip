@@ -18,6 +18,7 @@ struct DeviceScope {
     hipError_t error;
     explicit DeviceScope(int device) : now(device)
     {
+        (void)hipGetLastError();   // (what an earlier call of this thread left there is not this call's error)
         error = hipGetDevice(&before);
         if (error == hipSuccess && before != device) error = hipSetDevice(device);
     }

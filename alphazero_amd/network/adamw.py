@@ -7,7 +7,8 @@ It stands beside the momentum SGD of the reference's optimizer (network/main.py:
 `Network`'s training config.  The weight decay is AdamW's own, applied to the weight and not through the gradient.
 
 8-bit state: blocks of STATE_BLOCK elements, in the order in which they lie in memory, share one float32 scale s, the block's
-largest magnitude;  m = s sgn(c) (c / 127)^2 with c int8,  v = s (c / 255)^4 with c uint8 (at least 1 where v > 0).  The step
+largest magnitude;  m = s sgn(c) (c / 127)^2 with c int8,  v = s (c / 255)^4 with c uint8 (at least 1 where v > 0);  c is the nearest in
+the domain in which codes are evenly spaced, the even one of two that are equally near.  The step
 itself uses the new means before they are rounded to codes.  A block that holds an infinity or a NaN reads back as NaN.
 
 Tensors on the GPU go through the kernel, on PyTorch's current stream; tensors on the CPU take the same formulas in PyTorch.
@@ -24,8 +25,15 @@ def _blocks(n):
 
 
 def _companded(x, s, power, top):
-    s = s.double()
-    return torch.where(s > 0, (x.abs() / torch.where(s > 0, s, torch.ones_like(s))).pow(1.0 / power) * top, torch.zeros_like(x)).round().clamp(max=top)
+    """Codes of |x| <= s, x = s (c / top)^power with power 2 or 4: what the roots say, put right by comparing powers at the two
+    borders of that code."""
+    s, x = s.double(), x.abs()
+    root = torch.sqrt(x / torch.where(s > 0, s, torch.ones_like(s)))
+    c = ((torch.sqrt(root) if power == 4 else root) * top).round().clamp(max=top)
+    scaled, odd = x * (2.0 * top) ** power, c % 2 == 1
+    high, low = ((2 * c + 1) ** power) * s, torch.where(c > 0, ((2 * c - 1) ** power) * s, torch.full_like(x, -1.0))
+    up, down = (scaled > high) | ((scaled == high) & odd), (scaled < low) | ((scaled == low) & odd)
+    return torch.where(s > 0, (c + up.double() - down.double()).clamp(max=top), torch.zeros_like(x))
 
 
 def quantize_state(values, signed):

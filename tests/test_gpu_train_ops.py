@@ -294,6 +294,18 @@ def test_norm_two_threads_at_once():
     assert not bad
 
 
+def test_a_failed_call_leaves_nothing_behind():
+    """A device that does not exist is an error of that call only, and the current device stays."""
+    from alphazero_amd import _lib
+    L, x, y = _lib.lib(), torch.randn(4, 8, device=DEV), torch.empty(4, 8, device=DEV)
+    call = lambda device: L.az_layer_norm_fwd_dev(device, None, 0, 0, 4, 8, 1e-5, x.data_ptr(), 8, None, None, y.data_ptr(), 8, None, None, None, 0)  # noqa: E731
+    torch.cuda.synchronize()
+    assert call(999) == _lib.ERR_HIP and b"device" in L.az_last_error(None)
+    assert torch.cuda.current_device() == 0 and call(0) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y, layer_norm(x))
+
+
 # ---- AdamW ----------------------------------------------------------------------------------------------------------------
 HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.05)
 
@@ -362,6 +374,17 @@ def test_adamw_step(dtype, bits, step, fresh):
 @pytest.mark.parametrize("hyper", [dict(lr=0.0), dict(weight_decay=0.0), dict(betas=(0.0, 0.0)), dict(betas=(0.0, 0.99)), dict(eps=1.0), dict(lr=1.0, weight_decay=1.0)])
 def test_adamw_other_constants(bits, hyper):
     _check_step(_adamw_inputs(SHAPES, F32, bits, seed=5), 7, **dict(HYPER, **hyper))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("betas", [(0.9, 0.0), (0.0, 0.0), (0.0, 0.999)])
+def test_adamw_codes_on_a_border(dtype, betas):
+    """Without a memory of earlier steps the states of 16-bit gradients are squares and products of few bits, some of which lie
+    exactly between two codes."""
+    for seed in range(3):
+        args = _adamw_inputs([(20000,), (300,)], dtype, 8, seed=seed)
+        args[1][1] = (2.0 ** torch.randint(-6, 1, (300,), generator=_gen(seed), device=DEV)).to(dtype)      # g = gmax / 4: half of the root
+        _check_step(args, 3, **dict(HYPER, betas=betas))
 
 
 @pytest.mark.parametrize("bits", [32, 8])

@@ -118,6 +118,9 @@ def test_codes_are_the_nearest_and_read_back_as_themselves():
         codes, scales = A.quantize_state(x, signed)
         c, s = R.codes_of(x.double(), signed)
         assert torch.equal(codes, c) and torch.equal(scales, s)
+        g = (torch.randint(1, 257, (3000,)) * 2.0 ** torch.randint(-9, 1, (3000,)))
+        g = g if signed else g * g                  # few bits: some lie on a border between two codes
+        assert torch.equal(A.quantize_state(g, signed)[0], R.codes_of(g.double(), signed)[0])
         back = A.dequantize_state(codes, scales)
         again, _ = A.quantize_state(back, signed)
         assert torch.equal(again, codes) and back.dtype == F32

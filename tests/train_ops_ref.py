@@ -1,4 +1,6 @@
 """Layer norm and the AdamW step in 64 bits, written from their formulas, with bounds on what float32 arithmetic may be off by."""
+from fractions import Fraction
+
 import torch
 
 U32 = 2.0 ** -24          # half a step of float32, relative
@@ -81,10 +83,16 @@ def codes_of(x, signed):
     s = full.abs().amax(1).float()
     d = s.double()[:, None]
     ratio = torch.where((d > 0) & torch.isfinite(d), full.abs() / d, torch.zeros_like(full))
+    x = 127.0 * torch.sqrt(ratio) if signed else 255.0 * torch.sqrt(torch.sqrt(ratio))
+    c = x.round()
+    # what may lie on a border is settled in whole numbers: the even code where it does
+    for i, j in ((x - x.floor() - 0.5).abs() < 1e-9).nonzero().tolist():
+        value, scale, low = Fraction(abs(float(full[i, j]))), Fraction(float(s[i])), int(x[i, j])
+        border = scale * Fraction(2 * low + 1, 254 if signed else 510) ** (2 if signed else 4)
+        c[i, j] = low + (1 if value > border or (value == border and low % 2) else 0)
     if signed:
-        c = (127.0 * torch.sqrt(ratio)).round() * full.sign()
+        c = c * full.sign()
     else:
-        c = (255.0 * torch.sqrt(torch.sqrt(ratio))).round()
         c = torch.where((full > 0) & (d > 0) & torch.isfinite(d), c.clamp(min=1.0), c)
     return torch.nan_to_num(c).reshape(-1)[:n].to(torch.int8 if signed else torch.uint8), s
 
