@@ -289,7 +289,9 @@ struct NormBwd {
 // add up through LDS at the end.
 // Elements past a row's end need no masks: their dy reads as 0, so they add nothing to any sum, and they are not stored.
 // STREAM: x and dy, which this pass is the last to read, go past the L2 caches.
-template <typename T, int TPR, int NV, bool STREAM> __global__ __launch_bounds__(norm_threads(TPR)) void k_layer_norm_bwd(NormBwd a)
+// Without SUMS there is dx alone: a thread of a workgroup of 1024 has registers for 16 elements of x, dy and w, but not for
+// their sums too.
+template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __launch_bounds__(norm_threads(TPR)) void k_layer_norm_bwd(NormBwd a)
 {
     constexpr int N = Pack<T>::N, THREADS = norm_threads(TPR), GROUPS = THREADS / TPR, WIDTH = (TPR * NV + 1) * N;
     __shared__ float cell[2][2][16];
@@ -297,12 +299,14 @@ template <typename T, int TPR, int NV, bool STREAM> __global__ __launch_bounds__
     const int t = threadIdx.x % TPR, cols = (int)a.cols, packs = cols / N, last = packs * N + t;
     const bool tail = last < cols;
     const float inv = 1.0f / (float)cols;
-    float w[NV][N], dw[NV][N], db[NV][N], dw1 = 0.f, db1 = 0.f;
+    float w[NV][N], dw[SUMS ? NV : 1][N], db[SUMS ? NV : 1][N], dw1 = 0.f, db1 = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         load_affine_pack<T>(a.w, a.affine_f32, (k * TPR + t) * N, k * TPR + t < packs, 1.0f, w[k]);
+        if constexpr (SUMS) {
 #pragma unroll
-        for (int e = 0; e < N; e++) dw[k][e] = db[k][e] = 0.f;
+            for (int e = 0; e < N; e++) dw[k][e] = db[k][e] = 0.f;
+        }
     }
     const float w1 = load_affine_one<T>(a.w, a.affine_f32, last, tail, 1.0f);
     const int64_t step = (int64_t)gridDim.x * GROUPS;
@@ -344,8 +348,10 @@ template <typename T, int TPR, int NV, bool STREAM> __global__ __launch_bounds__
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                dw[k][e] += g[k][e] * h[k][e];
-                db[k][e] += g[k][e];
+                if constexpr (SUMS) {
+                    dw[k][e] += g[k][e] * h[k][e];
+                    db[k][e] += g[k][e];
+                }
                 g[k][e] *= w[k][e];
                 s[0] += g[k][e];
                 s[1] += g[k][e] * h[k][e];
@@ -366,12 +372,12 @@ template <typename T, int TPR, int NV, bool STREAM> __global__ __launch_bounds__
     }
     if (!a.part) return;
 #pragma unroll
-    for (int which = 0; which < 2; which++) {
+    for (int which = 0; which < (SUMS ? 2 : 0); which++) {
         float *part = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.cols;
         if constexpr (GROUPS == 1) {
 #pragma unroll
             for (int k = 0; k < NV; k++) {
-                const float *f = which ? db[k] : dw[k];
+                const float *f = which ? db[SUMS ? k : 0] : dw[SUMS ? k : 0];
                 if (k * TPR + t < packs) {
 #pragma unroll
                     for (int e = 0; e < N; e += 4) store4(part + (k * TPR + t) * N + e, make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]));
@@ -385,7 +391,7 @@ template <typename T, int TPR, int NV, bool STREAM> __global__ __launch_bounds__
             for (int k = 0; k < NV; k++) {
                 if (k * TPR + t < packs) {
 #pragma unroll
-                    for (int e = 0; e < N; e++) mine[(k * TPR + t) * N + e] = which ? db[k][e] : dw[k][e];
+                    for (int e = 0; e < N; e++) mine[(k * TPR + t) * N + e] = which ? db[SUMS ? k : 0][e] : dw[SUMS ? k : 0][e];
                 }
             }
             if (tail) mine[last] = which ? db1 : dw1;

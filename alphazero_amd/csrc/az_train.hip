@@ -34,10 +34,12 @@ int fail_hip(const char *what, hipError_t e)
 
 bool bad_type(int32_t t) { return t != AZ_TYPE_F32 && t != AZ_TYPE_BF16 && t != AZ_TYPE_F16; }
 
-// Whole 16-byte packs of a row.  The register forms hold up to 8192 elements in them, 8 to a thread of the largest workgroup
-// (16 would spill in the backward pass, which holds five numbers for each).
+// Whole 16-byte packs of a row.  The register forms hold up to 16384 elements in them, 16 to a thread of the largest workgroup.
 int64_t norm_packs(int64_t cols, int32_t type) { return cols / (type == AZ_TYPE_F32 ? 4 : 8); }
-bool norm_wide(int64_t cols, int32_t type) { return norm_packs(cols, type) > (type == AZ_TYPE_F32 ? 2048 : 1024); }
+bool norm_wide(int64_t cols, int32_t type) { return norm_packs(cols, type) > (type == AZ_TYPE_F32 ? 4096 : 2048); }
+
+// Above 8192 elements the backward pass has no registers left for the sums over the rows: a pass of their own.
+bool norm_sums_apart(int64_t cols, int32_t type) { return norm_packs(cols, type) > (type == AZ_TYPE_F32 ? 2048 : 1024); }
 
 // Threads per row and packs per thread: the narrowest form that holds the row, one wave up to 256 packs.  (At least as many
 // threads as there can be elements past the last whole pack.)  Forward, 1 M rows: 8 float32 columns 14 us with four threads to
@@ -54,8 +56,9 @@ template <typename T, typename Launch> void norm_form(int64_t packs, const Launc
     else if (packs <= 128) launch.template operator()<T, 64, 2>();
     else if (packs <= 256) launch.template operator()<T, 64, 4>();
     else if (packs <= 512) launch.template operator()<T, 512 / NV, NV>();
-    else if (packs <= 1024) launch.template operator()<T, 1024 / NV, NV>();
-    else if constexpr (NV == 2) launch.template operator()<T, 1024, 2>();
+    else if (packs <= 1024 && NV == 2) launch.template operator()<T, 1024 / NV, NV>();
+    else if (packs <= 1024 * NV) launch.template operator()<T, 1024, NV>();
+    else launch.template operator()<T, 1024, 2 * NV>();
 }
 
 // rows that a workgroup works on at a time, and its threads, by the same rule
@@ -80,8 +83,9 @@ bool norm_lines(int64_t cols, int32_t type) { return cols * (type == AZ_TYPE_F32
 int64_t norm_fwd_blocks(int64_t cols, int32_t type)
 {
     const int64_t packs = norm_packs(cols, type);
+    if (norm_sums_apart(cols, type)) return 256;          // (as many as its registers leave room for)
     if (packs > 256) return 256 * 2048 / norm_block(packs, type);
-    if (packs > 128 && type != AZ_TYPE_F32) return 768;   // (as many as its registers leave room for)
+    if (packs > 128 && type != AZ_TYPE_F32) return 768;   // (the same)
     return norm_lines(cols, type) ? 1024 : 2048;
 }
 
@@ -139,7 +143,7 @@ struct FwdType {
 int64_t bwd_parts(int64_t rows, int64_t cols, int32_t type)
 {
     if (rows <= 0) return 0;
-    if (norm_wide(cols, type)) return std::min<int64_t>(rows, 64);
+    if (norm_sums_apart(cols, type)) return std::min<int64_t>(rows, 64);
     const int64_t packs = norm_packs(cols, type), groups = norm_groups(packs, type), each = (rows + groups - 1) / groups;
     return std::min(norm_bwd_blocks(cols, type), std::max((each + 3) / 4, std::min<int64_t>(each, 64)));
 }
@@ -148,8 +152,13 @@ struct BwdForm {
     const NormBwd &a; hipStream_t st; int64_t parts;
     template <typename T, int TPR, int NV> void operator()() const
     {
-        if (a.stream) k_layer_norm_bwd<T, TPR, NV, true><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
-        else k_layer_norm_bwd<T, TPR, NV, false><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
+        if constexpr (TPR * NV * Pack<T>::N > 8192) {
+            const unsigned blocks = (unsigned)std::min<int64_t>(a.rows, 256);
+            if (!a.dx) return;
+            if (a.stream) k_layer_norm_bwd<T, TPR, NV, true, false><<<blocks, norm_threads(TPR), 0, st>>>(a);
+            else k_layer_norm_bwd<T, TPR, NV, false, false><<<blocks, norm_threads(TPR), 0, st>>>(a);
+        } else if (a.stream) k_layer_norm_bwd<T, TPR, NV, true, true><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
+        else k_layer_norm_bwd<T, TPR, NV, false, true><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
     }
 };
 struct BwdType {
@@ -158,17 +167,18 @@ struct BwdType {
     {
         const int64_t parts = bwd_parts(a.rows, a.cols, type);
         if (parts > 0) {
-            if (norm_wide(a.cols, type)) {
-                const int64_t chunks = norm_chunks(a.rows, a.cols, type);
-                if (a.dx && chunks) {
-                    const dim3 grid((unsigned)chunks, (unsigned)a.rows);
-                    k_layer_norm_chunk_sums<T><<<grid, AZ_NORM_WIDE_THREADS, 0, st>>>(a, part);
-                    k_layer_norm_chunk_dx<T><<<grid, AZ_NORM_WIDE_THREADS, 0, st>>>(a, part);
-                } else if (a.dx) k_layer_norm_bwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2 * 256), AZ_NORM_WIDE_THREADS, 0, st>>>(a);
-                if (a.part) k_layer_norm_cols_wide<T><<<dim3((unsigned)((a.cols + 1023) / 1024), (unsigned)parts), AZ_NORM_COLS_WIDE_THREADS, 0, st>>>(a);
-            } else {
+            const int64_t chunks = norm_chunks(a.rows, a.cols, type);
+            if (!norm_wide(a.cols, type)) {
                 norm_form<T>(norm_packs(a.cols, type), BwdForm{a, st, parts});
+            } else if (a.dx && chunks) {
+                const dim3 grid((unsigned)chunks, (unsigned)a.rows);
+                k_layer_norm_chunk_sums<T><<<grid, AZ_NORM_WIDE_THREADS, 0, st>>>(a, part);
+                k_layer_norm_chunk_dx<T><<<grid, AZ_NORM_WIDE_THREADS, 0, st>>>(a, part);
+            } else if (a.dx) {
+                k_layer_norm_bwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2 * 256), AZ_NORM_WIDE_THREADS, 0, st>>>(a);
             }
+            if (a.part && norm_sums_apart(a.cols, type))
+                k_layer_norm_cols_wide<T><<<dim3((unsigned)((a.cols + 1023) / 1024), (unsigned)parts), AZ_NORM_COLS_WIDE_THREADS, 0, st>>>(a);
         }
         if (dw || db)
             k_layer_norm_cols<T><<<dim3((unsigned)((a.cols + 15) / 16), 2), 1024, 0, st>>>(a.part, parts, a.cols, dw, db, a.affine_f32);

@@ -73,7 +73,8 @@ def test_norm_every_number_of_rows(rows, cols, dtype, affine):
     _check_norm(*_norm_case(rows, cols, dtype, affine, seed=rows))
 
 
-@pytest.mark.parametrize("rows,cols", [(3, 8193), (255, 8200), (256, 8200), (257, 12345), (3, 300000), (1, 1000001), (100, 24576), (2, 16384), (2, 16385)])
+@pytest.mark.parametrize("rows,cols", [(3, 8193), (255, 8200), (256, 8200), (257, 12345), (3, 300000), (1, 1000001), (100, 24576), (2, 16384), (2, 16385),
+                                       (2, 16387), (2, 16388), (2, 16391), (2, 16392), (255, 16392), (256, 16400), (300, 20000), (2000, 16384)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_norm_wide_rows_in_chunks(rows, cols, dtype):
     """Rows too wide for a workgroup, few of them (in chunks) and many."""
@@ -87,13 +88,13 @@ def test_norm_narrow_rows(cols, dtype):
         _check_norm(*_norm_case(rows, cols, dtype, F32, seed=cols))
 
 
-@pytest.mark.parametrize("cols", [20, 256, 3000, 9000])
+@pytest.mark.parametrize("cols", [20, 256, 3000, 9000, 20000])
 @pytest.mark.parametrize("weight,bias", [(False, False), (True, False), (False, True)])
 def test_norm_without_weight_or_bias(cols, weight, bias):
     _check_norm(*_norm_case(33, cols, F32, F32, seed=3, weight=weight, bias=bias))
 
 
-@pytest.mark.parametrize("cols", [20, 256, 3000, 9000])
+@pytest.mark.parametrize("cols", [20, 256, 3000, 9000, 20000])
 def test_norm_gradients_one_at_a_time(cols):
     x, w, b, dy = _norm_case(50, cols, F32, F32, seed=4)
     full = [t.detach().requires_grad_() for t in (x, w, b)]
@@ -104,13 +105,13 @@ def test_norm_gradients_one_at_a_time(cols):
         assert torch.equal(got, want[i])
 
 
-@pytest.mark.parametrize("cols", [48, 256, 700, 2500, 9000])
+@pytest.mark.parametrize("cols", [48, 256, 700, 2500, 9000, 20000])
 @pytest.mark.parametrize("offset", [100.0, 3000.0])
 def test_norm_rows_with_a_mean_far_from_zero(cols, offset):
     _check_norm(*_norm_case(40, cols, F32, F32, seed=5, offset=offset))
 
 
-@pytest.mark.parametrize("cols", [16, 256, 361, 5000, 9001])
+@pytest.mark.parametrize("cols", [16, 256, 361, 5000, 9001, 20001])
 def test_norm_strides(cols):
     g = _gen(6)
     w, b = 1 + 0.1 * torch.randn(cols, generator=g, device=DEV), torch.randn(cols, generator=g, device=DEV)
@@ -141,7 +142,7 @@ def test_norm_channels_of_an_image():
     _check_norm(x.permute(0, 2, 3, 1), torch.ones(256, device=DEV), torch.zeros(256, device=DEV), torch.randn(3, 9, 9, 256, generator=_gen(9), device=DEV))
 
 
-@pytest.mark.parametrize("cols", [8, 256, 9000])
+@pytest.mark.parametrize("cols", [8, 256, 9000, 20000])
 def test_norm_without_rows(cols):
     x = torch.empty(0, cols, device=DEV, requires_grad=True)
     w, b = torch.ones(cols, device=DEV, requires_grad=True), torch.zeros(cols, device=DEV, requires_grad=True)
@@ -150,7 +151,7 @@ def test_norm_without_rows(cols):
     assert y.shape == dx.shape == (0, cols) and not dw.any() and not db.any()
 
 
-@pytest.mark.parametrize("cols", [12, 200, 361, 3000, 9000])
+@pytest.mark.parametrize("cols", [12, 200, 361, 3000, 9000, 20000])
 def test_norm_values_that_are_not_finite_stay_in_their_row(cols):
     x, w, b, dy = _norm_case(9, cols, F32, F32, seed=10)
     good = layer_norm(x, w, b)
@@ -228,7 +229,7 @@ def test_norm_gradient_against_differences():
             assert abs((ends[0] - ends[1]) / (2 * e) - float(g.view(-1)[i])) < 5e-3
 
 
-@pytest.mark.parametrize("rows,cols", [(512, 722), (3, 20000), (300, 9000)])
+@pytest.mark.parametrize("rows,cols", [(512, 722), (3, 20000), (300, 9000), (300, 17000)])
 def test_norm_other_stream_and_capture(rows, cols):
     x, w, b, dy = _norm_case(rows, cols, F32, F32, seed=16)
     want = layer_norm(x, w, b)
