@@ -101,7 +101,7 @@ def adamw(p, g, m, v, step, lr, beta1, beta2, eps, decay):
     """New (p, m, v) and the bounds of float32 arithmetic on them; m and v as the values they stand for."""
     p, g, m, v = (t.double() for t in (p, g, m, v))
     m2 = beta1 * m + (1 - beta1) * g
-    v2 = beta2 * v + (1 - beta2) * g * g
+    v2 = beta2 * v + (1 - beta2) * (g * g)     # (rounded in the order in which the kernels document it)
     den = (v2 / (1 - beta2 ** step)) ** 0.5 + eps
     update = lr * (m2 / (1 - beta1 ** step)) / den
     p2 = p - lr * decay * p - update
