@@ -28,6 +28,7 @@ struct AdamwTable {
 struct AdamwScalars {
     double beta1, beta2, one_minus_beta1, one_minus_beta2;
     float decay, step_size, inv_sqrt_c2, eps;   // lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+    bool tiny;                                  // the root of a subnormal v is not negligible beside eps
 };
 static_assert(sizeof(AdamwTable) + sizeof(AdamwScalars) <= 4096, "kernel arguments");
 
@@ -39,12 +40,18 @@ __device__ __forceinline__ int adamw_tensor(const AdamwTable &a, uint32_t block)
 }
 
 // Square root and reciprocal by the instructions that are right to one step of float32, a third of the work of the correctly
-// rounded ones: their error is in the update, not in the weight.  They take no subnormal numbers, so a tiny v is scaled.
-__device__ __forceinline__ float adamw_weight(float w, float m, float v, const AdamwScalars &k)
+// rounded ones: their error is in the update, not in the weight.  They take no subnormal numbers: a v below 2^-126 counts as
+// nothing beside eps, or, where eps is so small that it does not (k.tiny), is scaled.
+__device__ __forceinline__ float adamw_root(float v, const AdamwScalars &k)
 {
+    if (!k.tiny) return __builtin_amdgcn_sqrtf(v);
     const bool small = v < 0x1p-96f;
-    const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? k.inv_sqrt_c2 * 0x1p-32f : k.inv_sqrt_c2);
-    return fmaf(-k.step_size * m, __builtin_amdgcn_rcpf(root + k.eps), fmaf(-k.decay, w, w));
+    return __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? 0x1p-32f : 1.0f);
+}
+
+__device__ __forceinline__ float adamw_weight(float w, float m, float root, const AdamwScalars &k)
+{
+    return fmaf(-k.step_size * m, __builtin_amdgcn_rcpf(fmaf(root, k.inv_sqrt_c2, k.eps)), fmaf(-k.decay, w, w));
 }
 
 // (which products are fused is written out: a tensor's result does not depend on the form of the kernel that its size selects)
@@ -52,7 +59,7 @@ __device__ __forceinline__ void adamw_32(float &w, float g, float &m, float &v, 
 {
     m = fmaf((float)k.beta1, m, (float)k.one_minus_beta1 * g);
     v = fmaf((float)k.beta2, v, (float)k.one_minus_beta2 * (g * g));
-    w = adamw_weight(w, m, v, k);
+    w = adamw_weight(w, m, adamw_root(v, k), k);
 }
 
 // What a workgroup works on: TURNS * 1024 neighbouring elements of one tensor, `left` of them before its end.
@@ -123,8 +130,8 @@ template <typename T, int TURNS, bool STREAM> __global__ __launch_bounds__(AZ_AD
 // multiply-add): b1 S + (1 - b1) g lies exactly between two float32 values in one block of a hundred, and the scale must not
 // depend on how a compiler contracts the sum.
 // Codes are those of the 64-bit means too: a value next to a border between two codes goes to the right side of it.  A
-// float32 estimate of 127 sqrt(|m| / S) or 255 (v / S)^(1/4) is off by less than 1e-4 (one step each of the conversion, the
-// reciprocal, two roots and the products), so only what it puts within 2e-4 of a border, one wave in eight, is compared with
+// float32 estimate of 127 sqrt(|m| / S) or 255 sqrt(sqrt(v) / sqrt(S)) is off by less than 1e-4 (one step each of the conversion,
+// the reciprocal, the roots and the products), so only what it puts within 2e-4 of a border, one wave in eight, is compared with
 // that border, by powers and without roots: (2c - 1)^2 S < 254^2 |m| < (2c + 1)^2 S.  A value on a border goes to the even code
 // (with b2 = 0 and 16-bit gradients that happens: both sides of the comparison round the same product then, and are equal).  With that, 95 M bfloat16 parameters take
 // 193 us (950 MB, 4.9 TB/s); with the comparison for every element they took 360 us and were bound by arithmetic.
@@ -162,20 +169,21 @@ __device__ __forceinline__ float border_v(double v, double s, double inv)
     return (float)min(c + (t > hi || (t == hi && odd) ? 1 : 0) - (t < lo || (t == lo && odd) ? 1 : 0), 255);
 }
 
-// four codes as the bytes of a word; `bits` are the scale's, the same in the whole wave
+// Four codes as the bytes of a word; `bits` are the scale's, the same in the whole wave.  v comes with its root, which the
+// update has needed already.
 __device__ __forceinline__ uint32_t quantize_m(const double (&m)[4], const float (&f)[4], uint32_t bits)
 {
     if (bits == 0 || bits >= 0x7f800000u) return 0;
     const float s = __uint_as_float(bits), inv = __builtin_amdgcn_rcpf(s);
-    bool near = s < 0x1p-100f || s > 0x1p100f;   // where the reciprocal is no longer a normal number, or close to it
-    float c[4];
+    float c[4], off = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const float x = 127.0f * __builtin_amdgcn_sqrtf(fabsf(f[e]) * inv);
         c[e] = rintf(x);
-        near |= fabsf(x - c[e]) > 0.4998f;
+        off = fmaxf(off, fabsf(x - c[e]));
     }
-    if (near) {
+    // (also where the reciprocal is no longer a normal number, or close to it)
+    if (off > 0.4998f || s < 0x1p-100f || s > 0x1p100f) {
         const double d = (double)s, dinv = 1.0 / d;
 #pragma unroll
         for (int e = 0; e < 4; e++) c[e] = border_m(m[e], d, dinv);
@@ -186,19 +194,19 @@ __device__ __forceinline__ uint32_t quantize_m(const double (&m)[4], const float
     return w ^ 0x80808080u;
 }
 
-__device__ __forceinline__ uint32_t quantize_v(const double (&v)[4], const float (&f)[4], uint32_t bits)
+__device__ __forceinline__ uint32_t quantize_v(const double (&v)[4], const float (&root)[4], uint32_t bits)
 {
     if (bits == 0 || bits >= 0x7f800000u) return 0;
-    const float s = __uint_as_float(bits), inv = __builtin_amdgcn_rcpf(s);
-    bool near = s < 0x1p-100f || s > 0x1p100f;
-    float c[4];
+    const float s = __uint_as_float(bits), inv = __builtin_amdgcn_rsqf(s);
+    float c[4], off = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const float x = 255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(f[e] * inv));
+        const float x = 255.0f * __builtin_amdgcn_sqrtf(root[e] * inv);
         c[e] = rintf(x);
-        near |= fabsf(x - c[e]) > 0.4998f;
+        off = fmaxf(off, fabsf(x - c[e]));
     }
-    if (near) {
+    // (also where a subnormal v, whose root may read as 0, is not yet a code of 0)
+    if (off > 0.4998f || s < 0x1p-60f || s > 0x1p100f) {
         const double d = (double)s, dinv = 1.0 / d;
 #pragma unroll
         for (int e = 0; e < 4; e++) c[e] = border_v(v[e], d, dinv);
@@ -230,8 +238,6 @@ template <bool FULL> __device__ __forceinline__ void store_codes(uint8_t *p, int
     if (i + 2 < n) p[i + 2] = (uint8_t)(w >> 16);
 }
 
-__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
 // A workgroup's chunk in blocks of 256, one for each of its waves at a time.
 template <typename T, int TURNS, bool STREAM, bool FULL> __device__ __forceinline__ void adamw_8_chunk(const AdamwTable &a, const AdamwScalars &k, const AdamwChunk &ch)
 {
@@ -259,7 +265,7 @@ template <typename T, int TURNS, bool STREAM, bool FULL> __device__ __forceinlin
         float *we = reinterpret_cast<float *>(&w[u]);
         const float *ge = reinterpret_cast<const float *>(&g[u]);
         double m[4], v[4];
-        float mf[4], vf[4];
+        float mf[4], root[4];
         uint32_t mb = 0, vb = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -268,15 +274,16 @@ template <typename T, int TURNS, bool STREAM, bool FULL> __device__ __forceinlin
             m[e] = k.beta1 * dequantize_m(signed_code(mc[u], e), (double)ms[u]) + k.one_minus_beta1 * gd;
             v[e] = k.beta2 * dequantize_v(unsigned_code(vc[u], e), (double)vs[u]) + k.one_minus_beta2 * (gd * gd);
             mf[e] = (float)m[e];
-            vf[e] = (float)v[e];
-            mb = max(mb, magnitude_bits(mf[e]));
-            vb = max(vb, magnitude_bits(vf[e]));
+            const float vf = (float)v[e];
+            mb = max(mb, __float_as_uint(mf[e]) & 0x7fffffffu);
+            vb = max(vb, __float_as_uint(vf));     // (never negative)
+            root[e] = adamw_root(vf, k);
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) we[e] = adamw_weight(we[e], mf[e], vf[e], k);
+        for (int e = 0; e < 4; e++) we[e] = adamw_weight(we[e], mf[e], root[e], k);
         // NaN has the largest magnitude bits of all, so the integer maximum keeps it
         mb = wave_umax(mb); vb = wave_umax(vb);
-        const uint32_t mw = quantize_m(m, mf, mb), vw = quantize_v(v, vf, vb);
+        const uint32_t mw = quantize_m(m, mf, mb), vw = quantize_v(v, root, vb);
         adamw_store<FULL, STREAM>(wp, at, n, w[u]);
         store_codes<FULL>(mp, at, n, mw); store_codes<FULL>(vp, at, n, vw);
         if ((threadIdx.x & 63) == 0 && (FULL || block * AZ_ADAMW_BLOCK < n)) {

@@ -372,7 +372,7 @@ def test_adamw_step(dtype, bits, step, fresh):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("hyper", [dict(lr=0.0), dict(weight_decay=0.0), dict(betas=(0.0, 0.0)), dict(betas=(0.0, 0.99)), dict(eps=1.0), dict(lr=1.0, weight_decay=1.0)])
+@pytest.mark.parametrize("hyper", [dict(lr=0.0), dict(weight_decay=0.0), dict(betas=(0.0, 0.0)), dict(betas=(0.0, 0.99)), dict(eps=1.0), dict(eps=1e-12), dict(eps=0.0), dict(lr=1.0, weight_decay=1.0)])
 def test_adamw_other_constants(bits, hyper):
     _check_step(_adamw_inputs(SHAPES, F32, bits, seed=5), 7, **dict(HYPER, **hyper))
 
@@ -474,6 +474,31 @@ def test_adamw_zero_gradients_and_no_history():
         before = [t.clone() for t in args[0]]
         _step_all(args, 1, **dict(HYPER, weight_decay=0.0))
         assert all(torch.equal(p, q) for p, q in zip(args[0], before)) and not any(t.any() for k in (2, 3, 4, 5) for t in args[k])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-8, 1e-20, 1e-30])
+@pytest.mark.parametrize("size", [1e-12, 1e-16, 3e-17, 1e-18])
+def test_adamw_squares_near_the_smallest_numbers(bits, eps, size):
+    """v from 1e-24 down into the subnormal numbers (below 1.2e-38), with an eps beside which its root counts or does not; blocks
+    that hold values of very different size.  A subnormal v is itself only right to half of its last place, 2^-150."""
+    for mix in (1.0, 1e-3):
+        args = _adamw_inputs([(3000,)], F32, bits, seed=45, fresh=True)
+        g = torch.randn(3000, generator=_gen(46), device=DEV) * size
+        g[::3] *= mix
+        args[1] = [g]
+        old = args[0][0].clone()
+        _step_all(args, 2, **dict(HYPER, eps=eps))
+        want, m2, v2, tol, _, _ = R.adamw(old, g, torch.zeros(3000, device=DEV), torch.zeros(3000, device=DEV), 2, HYPER["lr"], 0.9, 0.999, eps, HYPER["weight_decay"])
+        root, den = (v2 / (1 - 0.999 ** 2)) ** 0.5, (v2 / (1 - 0.999 ** 2)) ** 0.5 + eps
+        lost = 1.0 - ((v2 - 2.0 ** -149).clamp(min=0.0) / v2.clamp(min=1e-300)) ** 0.5        # of the root, relative
+        tol = tol + (old.double() - want).abs() * (root * lost / (den - root * lost).clamp(min=1e-300)).clamp(max=1e6)
+        seen = v2 > 2.0 ** -148
+        assert bool(((args[0][0].double() - want).abs() <= tol)[seen].all())
+        if bits == 8:
+            for k, new, signed in ((2, m2, True), (3, v2, False)):
+                codes, scales = R.codes_of(new, signed)
+                assert torch.equal(args[k][0], codes) and torch.equal(args[k + 2][0], scales)
 
 
 def test_adamw_tiny_values():
