@@ -134,7 +134,7 @@ template <typename T, int TURNS, bool STREAM> __global__ __launch_bounds__(AZ_AD
 // the reciprocal, the roots and the products), so only what it puts within 2e-4 of a border, one wave in eight, is compared with
 // that border, by powers and without roots: (2c - 1)^2 S < 254^2 |m| < (2c + 1)^2 S.  A value on a border goes to the even code
 // (with b2 = 0 and 16-bit gradients that happens: both sides of the comparison round the same product then, and are equal).  With that, 95 M bfloat16 parameters take
-// 193 us (950 MB, 4.9 TB/s); with the comparison for every element they took 360 us and were bound by arithmetic.
+// 180 to 192 us (950 MB, 5.0 to 5.3 TB/s); with the comparison for every element they took 360 us and were bound by arithmetic.
 // A block with an infinity or a NaN in it has a scale that is not finite and reads back as NaN as a whole.
 
 // byte e of a word as int8 / uint8, in float32: c |c| and c^2 are exact there
