@@ -87,9 +87,20 @@ class NNEvaluator:
         """planes int8 (B,17,H,W) -> (priors float32 (B,O), values float32 (B,)): Network.response."""
         if self._eng is not None:
             return self._eng.tower_forward(planes)
+        return self._forward(self._net, planes)
+
+    def _forward(self, net, planes):
         with torch.no_grad():
-            p, v, _ = self._net(torch.as_tensor(np.asarray(planes), dtype=torch.float32, device=self._device))
+            p, v, _ = net(torch.as_tensor(np.asarray(planes), dtype=torch.float32, device=self._device))
         return p.cpu().numpy(), v.cpu().numpy()
+
+    def frozen(self):
+        """eval_batch with the weights of this moment, whatever load / set_weights bring later: what an engine's own copy of the
+        tower's weights is for a network that the tower holds (which has no use for this)."""
+        if self._eng is not None:
+            raise ValueError("the weights of a tower are held by the engine that loads them")
+        net = self._net     # (never written to again: _refold makes another one)
+        return lambda planes: self._forward(net, planes)
 
     def load(self, filename):
         self.rwlock.w_acquire()

@@ -157,8 +157,8 @@ class BatchedSelfplay:
     for all of them - finished slots are not re-armed until every game in flight has ended, then the weights are
     loaded and all slots start again, so no game ever sees two networks.
 
-    A network that the tower cannot hold (layer norm) is evaluated through nn_eval.eval_batch, once per round for all
-    games together, with the planes and priors passing through host memory.
+    A network that the tower cannot hold (layer norm) is evaluated through nn_eval.frozen(), once per round for all
+    games together, with the planes and priors passing through host memory; new weights come to it by the same rules.
 
     rng_streams: optional list of (transform ids, gamma draws, uniforms), one per slot - the engine then replays these
     draws instead of using its own generator (parity tests)."""
@@ -183,6 +183,7 @@ class BatchedSelfplay:
         self._nn_eval = nn_eval
         self._tower = hasattr(nn_eval, "_tower_blob")
         self._version = None
+        self._evaluate = None                   # (without a tower) the network of self._version
         self._replay = Engine(n_slots=self.REPLAY_SLOTS, device=device, **kw)
         self.n_games = n_games
         self._started = False
@@ -193,10 +194,14 @@ class BatchedSelfplay:
         self.last_slots = []                    # slot of every game the last run() returned
 
     def _sync_weights(self):
-        if self._version != self._nn_eval.version:
+        # (read before the weights: what another thread brings meanwhile is a newer version at the next poll)
+        version = self._nn_eval.version
+        if self._version != version:
             if self._tower:
                 self.eng.tower_load(self._nn_eval._tower_blob)
-            self._version = self._nn_eval.version
+            else:
+                self._evaluate = self._nn_eval.frozen()
+            self._version = version
 
     def _convert(self, popped):
         out = []
@@ -211,7 +216,7 @@ class BatchedSelfplay:
         for _ in range(n):
             if self.eng.selfplay_select() == 0:
                 break
-            self.eng.selfplay_finish(*self._nn_eval.eval_batch(self.eng.leaf_batch()[0]))
+            self.eng.selfplay_finish(*self._evaluate(self.eng.leaf_batch()[0]))
 
     def _watch_pool(self):
         grow_pool_when_used(self.eng, self.POOL_GROW_AT)
