@@ -287,7 +287,8 @@ struct NormBwd {
 // dx of the rows, and for every workgroup the sums of dy * h and dy over its rows in the order in which it meets them: no
 // atomics, so the same call gives the same bits.  The threads of a workgroup that hold the same columns of different rows
 // add up through LDS at the end.
-// Elements past a row's end need no masks: their dy reads as 0, so they add nothing to any sum, and they are not stored.
+// Elements past a row's end read as dy = 0 and have h = 0, so they add nothing to any sum, and they are not stored.  (Their h is
+// set and not left as -mean r: in a row without spread r is 1 / sqrt(eps), so that can overflow, and 0 times infinity is NaN.)
 // STREAM: x and dy, which this pass is the last to read, go past the L2 caches.
 // Without SUMS there is dx alone: a thread of a workgroup of 1024 has registers for 16 elements of x, dy and w, but not for
 // their sums too.
@@ -297,7 +298,7 @@ template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __laun
     __shared__ float cell[2][2][16];
     __shared__ float gather[GROUPS > 1 ? GROUPS * WIDTH : 1];
     const int t = threadIdx.x % TPR, cols = (int)a.cols, packs = cols / N, last = packs * N + t;
-    const bool tail = last < cols;
+    const bool full = packs == TPR * NV, tail = last < cols;
     const float inv = 1.0f / (float)cols;
     float w[NV][N], dw[SUMS ? NV : 1][N], db[SUMS ? NV : 1][N], dw1 = 0.f, db1 = 0.f;
 #pragma unroll
@@ -333,12 +334,18 @@ template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __laun
     int turn = 0;
     for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += step, row += step, turn ^= 1) {
         const float mean = next_mean, r = next_r;
-        const float h1 = ((float)next_x1 - mean) * r;
+        const float h1 = tail ? ((float)next_x1 - mean) * r : 0.f;
         float h[NV][N], g[NV][N], g1 = (float)next_dy1;
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int e = 0; e < N; e++) { h[k][e] = ((float)next_x[k][e] - mean) * r; g[k][e] = (float)next_dy[k][e]; }
+        if (!full) {
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int e = 0; e < N; e++) h[k][e] = k * TPR + t < packs ? h[k][e] : 0.f;
+        }
         if (first + step < a.rows) ask(row + step);
         dw1 += g1 * h1;
         db1 += g1;
