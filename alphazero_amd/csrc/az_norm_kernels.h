@@ -4,9 +4,11 @@
 //   dx = r * (g - mean(g) - h * mean(g * h)),  g = w * dy,  h = (x - mean) * r
 //   dw = sum over rows of dy * h,   db = sum over rows of dy
 //
-// All sums are float32 whatever the elements' type.  The variance is taken from the row's values less their mean, in
-// registers, in a second pass over those registers: a sum of squares would lose everything in rows whose mean is large
-// against their spread.
+// All sums are float32 whatever the elements' type.  What is summed for the mean is the row's values less its first one, and for
+// the variance those less their mean, in a second pass over the registers: sums of the values themselves, or of their squares,
+// are rounded in proportion to the mean and lose everything in rows whose mean is large against their spread (1000.1 in 361
+// columns: a mean one step off, and with it h = 0.02 in a row without any spread).
+// The mean that is kept for the backward pass is rounded to float32 once, which moves h by up to half its last place times r.
 //
 // A row belongs to TPR threads (4 to 32: part of a wave, 64: a wave, more: a workgroup), each of which holds NV packs of 16
 // bytes of it in registers, so a row is read from memory once; the up to 3 or 7 elements past the last whole pack are held one
@@ -60,19 +62,14 @@ template <int TPR, int N> __device__ __forceinline__ void group_sum(float (&v)[N
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            float s[WAVES];
-#pragma unroll
-            for (int j = 0; j < WAVES; j++) s[j] = cell[slot][i][j];
-#pragma unroll
-            for (int d = WAVES / 2; d > 0; d >>= 1)
-#pragma unroll
-                for (int j = 0; j < d; j++) s[j] += s[j + d];
-            v[i] = s[0];
+            // (by the lanes of a row: as many values to each thread as there are waves cost registers, and with them workgroups)
+            const float x = cell[slot][i][threadIdx.x & (WAVES - 1)];
+            v[i] = WAVES == 4 ? quad_sum(x) : WAVES == 8 ? oct_sum(x) : row16_sum(x);
         }
     }
 }
 
-// s / n, exact where the quotient is: rows of one value come out with exactly that mean
+// s / n to half a step
 __device__ __forceinline__ float mean_of(float s, float n, float inv)
 {
     const float q = s * inv;
@@ -81,6 +78,35 @@ __device__ __forceinline__ float mean_of(float s, float n, float inv)
 
 // 1 / sqrt(t) to one step of float32; the instruction takes no subnormal numbers
 __device__ __forceinline__ float inv_sqrt(float t) { return t < 0x1p-126f ? 1.0f / sqrtf(t) : __builtin_amdgcn_rsqf(t); }
+
+// How a row's values are taken relative to its first one: d = x scale - first.  The difference of two values overflows only in
+// rows of the largest numbers, which are scaled down: 2^25 of them, of either sign, then have a sum.  (A first value below
+// 2^102 is less than half a step of the largest number and takes nothing past it.)  The variance of such a row is infinite in
+// float32 unless it is 0.
+struct RowShift {
+    float scale, first;
+    __device__ __forceinline__ explicit RowShift(float x0) : scale(fabsf(x0) < 0x1p102f ? 1.0f : 0x1p-30f), first(x0 * scale) {}
+    __device__ __forceinline__ float operator()(float x) const { return fmaf(x, scale, -first); }
+    __device__ __forceinline__ float back() const { return scale == 1.0f ? 1.0f : 0x1p30f; }
+    __device__ __forceinline__ float value(float d) const { return fmaf(d, back(), first * back()); }   // the x whose d this is
+};
+
+// a value that all lanes of a wave hold alike, in a scalar register
+__device__ __forceinline__ float of_wave(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+
+// The first lane's value in each lane of groups of TPR lanes (as a load of its own for every row it took 30 us and not 28 for
+// 1 M rows of 32 bfloat16 columns).
+template <int TPR> __device__ __forceinline__ float first_lane(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    if constexpr (TPR == 4) return __uint_as_float(dpp_row<AZ_QUAD_FIRST>(u));
+    else if constexpr (TPR == 8) return __uint_as_float((threadIdx.x & 8) ? dpp_row<AZ_ROW_LANE(8)>(u) : dpp_row<AZ_ROW_LANE(0)>(u));
+    else if constexpr (TPR == 16) return __uint_as_float(dpp_row<AZ_ROW_LANE(0)>(u));
+    else if constexpr (TPR == 32) {
+        const uint32_t first = dpp_row<AZ_ROW_LANE(0)>(u);
+        return __uint_as_float(__builtin_amdgcn_permlane16_swap(first, first, false, false)[0]);    // of the even row of a pair
+    } else return of_wave(x);
+}
 
 struct NormFwd {
     const void *x, *w, *b;
@@ -96,7 +122,7 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads
     constexpr int N = Pack<T>::N, GROUPS = norm_threads(TPR) / TPR;
     __shared__ float cell[2][1][16];
     const int t = threadIdx.x % TPR, cols = (int)a.cols, packs = cols / N, last = packs * N + t;
-    const bool full = packs == TPR * NV, tail = last < cols;
+    const bool tail = last < cols;
     const float n = (float)cols, inv = 1.0f / n;
     float w[NV][N], b[NV][N];
 #pragma unroll
@@ -106,9 +132,10 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads
     }
     const float w1 = load_affine_one<T>(a.w, a.affine_f32, last, tail, 1.0f), b1 = load_affine_one<T>(a.b, a.affine_f32, last, tail, 0.0f);
     const int64_t step = (int64_t)gridDim.x * GROUPS;
-    int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
+    const int group = threadIdx.x / TPR;
+    int64_t row = (int64_t)blockIdx.x * GROUPS + (TPR < 64 ? group : __builtin_amdgcn_readfirstlane(group));
     typename Pack<T>::type next[NV];
-    T next1;
+    T next1, next0;
     // a row past the end reads as zeros
     const auto ask = [&](int64_t i) {
         const T *x = static_cast<const T *>(a.x) + i * a.x_stride;
@@ -117,35 +144,38 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads
             next[k] = {};
             if (i < a.rows && k * TPR + t < packs) next[k] = load_pack<false>(x + (k * TPR + t) * N);
         }
-        next1 = T(0);
+        next1 = next0 = T(0);
         if (i < a.rows && tail) next1 = x[last];
+        if (TPR > 64 && i < a.rows) next0 = x[0];
     };
     ask(row);
     // the number of turns is the same for every thread of a workgroup
-    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += step, row += step) {
-        float v[NV][N], v1 = (float)next1, s[1] = {v1}, q[1];
+    for (int64_t first_row = (int64_t)blockIdx.x * GROUPS; first_row < a.rows; first_row += step, row += step) {
+        // (with a wave or less to a row its first lane holds it, in the first pack or, if there is none, past it)
+        RowShift shift(TPR > 64 ? (float)next0 : first_lane<TPR>(packs ? (float)next[0][0] : (float)next1));
+        if constexpr (TPR >= 64) { shift.scale = of_wave(shift.scale); shift.first = of_wave(shift.first); }
+        // (packs past a row's end are zeros, and stay so if nothing is taken from them)
+        float v[NV][N], v1 = tail ? shift((float)next1) : 0.f, s[1] = {v1}, q[1];
 #pragma unroll
-        for (int k = 0; k < NV; k++)
+        for (int k = 0; k < NV; k++) {
+            const float first = k * TPR + t < packs ? shift.first : 0.f;
 #pragma unroll
-            for (int e = 0; e < N; e++) v[k][e] = (float)next[k][e];
-        if (first + step < a.rows) ask(row + step);
+            for (int e = 0; e < N; e++) v[k][e] = fmaf((float)next[k][e], shift.scale, -first);
+        }
+        if (first_row + step < a.rows) ask(row + step);
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int e = 0; e < N; e += 4) s[0] += (v[k][e] + v[k][e + 1]) + (v[k][e + 2] + v[k][e + 3]);
         group_sum<TPR>(s, cell, 0);
-        const float mean = mean_of(s[0], n, inv);
+        const float mean = mean_of(s[0], n, inv);     // of the row's values less its first
         v1 = tail ? v1 - mean : 0.f;
         q[0] = v1 * v1;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
+        for (int k = 0; k < NV; k++) {
+            const float centre = k * TPR + t < packs ? mean : 0.f;
 #pragma unroll
-            for (int e = 0; e < N; e++) v[k][e] -= mean;
-        if (!full) {
-#pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int e = 0; e < N; e++) v[k][e] = k * TPR + t < packs ? v[k][e] : 0.f;
+            for (int e = 0; e < N; e++) v[k][e] -= centre;
         }
 #pragma unroll
         for (int k = 0; k < NV; k++)
@@ -153,17 +183,17 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads
             for (int e = 0; e < N; e += 4)
                 q[0] += (v[k][e] * v[k][e] + v[k][e + 1] * v[k][e + 1]) + (v[k][e + 2] * v[k][e + 2] + v[k][e + 3] * v[k][e + 3]);
         group_sum<TPR>(q, cell, 1);
-        const float r = inv_sqrt(q[0] * inv + a.eps);
+        const float r = inv_sqrt(q[0] * inv * (shift.back() * shift.back()) + a.eps), rs = r * shift.back();
         if (row < a.rows) {
             T *y = static_cast<T *>(a.y) + row * a.y_stride;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
 #pragma unroll
-                for (int e = 0; e < N; e++) v[k][e] = v[k][e] * r * w[k][e] + b[k][e];
+                for (int e = 0; e < N; e++) v[k][e] = v[k][e] * rs * w[k][e] + b[k][e];
                 if (k * TPR + t < packs) store_pack(y + (k * TPR + t) * N, v[k], a.stream);
             }
-            if (tail) y[last] = (T)(v1 * r * w1 + b1);
-            if (a.mean && t == 0) { a.mean[row] = mean; a.rstd[row] = r; }
+            if (tail) y[last] = (T)(v1 * rs * w1 + b1);
+            if (a.mean && t == 0) { a.mean[row] = shift.value(mean); a.rstd[row] = r; }
         }
     }
 }
@@ -181,6 +211,21 @@ __device__ __forceinline__ float block_sum(float x, float *cell)
     return s;
 }
 
+// Elements c .. c+3 of a row of n as `shift` takes them, less `mean`; 0 past the row's end.
+__device__ __forceinline__ float4 shifted(float4 v, const RowShift &shift, float mean, int64_t c, int64_t n)
+{
+    const float4 d = make_float4(shift(v.x) - mean, shift(v.y) - mean, shift(v.z) - mean, shift(v.w) - mean);
+    if (c + 4 <= n) return d;
+    return make_float4(c < n ? d.x : 0.f, c + 1 < n ? d.y : 0.f, c + 2 < n ? d.z : 0.f, 0.f);
+}
+template <typename T> __device__ __forceinline__ float4 shifted(const T *x, const RowShift &shift, float mean, int64_t c, int64_t n)
+{
+    if (c + 4 <= n) return shifted(load4(x + c), shift, mean, 0, 4);
+    return shifted(load4(x, c, n), shift, mean, c, n);
+}
+
+__device__ __forceinline__ float squares(float4 d) { return (d.x * d.x + d.y * d.y) + (d.z * d.z + d.w * d.w); }
+
 // Rows too wide for a workgroup's registers: read three times, the second and third time from cache.
 template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_layer_norm_fwd_wide(NormFwd a)
 {
@@ -190,29 +235,23 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
         T *y = static_cast<T *>(a.y) + row * a.y_stride;
+        const RowShift shift((float)x[0]);
         float s = 0.f, q = 0.f;
-        for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) s += sum4(load4(x, c, a.cols));
+        for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) s += sum4(shifted(x, shift, 0.f, c, a.cols));
         const float mean = mean_of(block_sum(s, cell), (float)a.cols, inv);
+        for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) q += squares(shifted(x, shift, mean, c, a.cols));
+        const float r = inv_sqrt(block_sum(q, cell) * inv * (shift.back() * shift.back()) + a.eps), rs = r * shift.back();
         for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) {
-            const float4 v = load4(x, c, a.cols);
-            const float d0 = v.x - mean, d1 = v.y - mean, d2 = v.z - mean, d3 = v.w - mean;
-            q += d0 * d0;
-            if (c + 1 < a.cols) q += d1 * d1;
-            if (c + 2 < a.cols) q += d2 * d2;
-            if (c + 3 < a.cols) q += d3 * d3;
-        }
-        const float r = inv_sqrt(block_sum(q, cell) * inv + a.eps);
-        for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) {
-            const float4 v = load4(x, c, a.cols), w = load_affine<T>(a.w, a.affine_f32, c, a.cols, 1.0f);
+            const float4 v = shifted(x, shift, mean, c, a.cols), w = load_affine<T>(a.w, a.affine_f32, c, a.cols, 1.0f);
             const float4 b = load_affine<T>(a.b, a.affine_f32, c, a.cols, 0.0f);
-            store4(y, c, a.cols, make_float4((v.x - mean) * r * w.x + b.x, (v.y - mean) * r * w.y + b.y, (v.z - mean) * r * w.z + b.z, (v.w - mean) * r * w.w + b.w));
+            store4(y, c, a.cols, make_float4(v.x * rs * w.x + b.x, v.y * rs * w.y + b.y, v.z * rs * w.z + b.z, v.w * rs * w.w + b.w));
         }
-        if (a.mean && threadIdx.x == 0) { a.mean[row] = mean; a.rstd[row] = r; }
+        if (a.mean && threadIdx.x == 0) { a.mean[row] = shift.value(mean); a.rstd[row] = r; }
     }
 }
 
 // A few rows that are too wide: a workgroup to a chunk of 8192 elements, in two launches.  The first leaves each chunk's mean
-// and its sum of squared distances from that mean; the second puts them together,
+// (relative to the row's first value) and its sum of squared distances from that mean; the second puts them together,
 //   mean = sum n_i mean_i / n,   sum of squares = sum (M2_i + n_i (mean_i - mean)^2),
 // and writes its chunk.  3 rows of 300 k float32: 18 us, with a workgroup to each row 72.
 #define AZ_NORM_CHUNK 8192
@@ -226,20 +265,16 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
     constexpr int NV = AZ_NORM_CHUNK / (AZ_NORM_WIDE_THREADS * 4);
     const T *x = static_cast<const T *>(a.x) + blockIdx.y * a.x_stride;
     const float n = (float)min((int64_t)AZ_NORM_CHUNK, a.cols - (int64_t)blockIdx.x * AZ_NORM_CHUNK);
+    const RowShift shift((float)x[0]);
     float4 v[NV];
     float s = 0.f, q = 0.f;
 #pragma unroll
-    for (int k = 0; k < NV; k++) { v[k] = load4(x, chunk_at(k), a.cols); s += sum4(v[k]); }
+    for (int k = 0; k < NV; k++) v[k] = load4(x, chunk_at(k), a.cols);
+#pragma unroll
+    for (int k = 0; k < NV; k++) s += sum4(shifted(v[k], shift, 0.f, chunk_at(k), a.cols));
     const float mean = mean_of(block_sum(s, cell), n, 1.0f / n);
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        const int64_t c = chunk_at(k);
-        const float d0 = v[k].x - mean, d1 = v[k].y - mean, d2 = v[k].z - mean, d3 = v[k].w - mean;
-        if (c < a.cols) q += d0 * d0;
-        if (c + 1 < a.cols) q += d1 * d1;
-        if (c + 2 < a.cols) q += d2 * d2;
-        if (c + 3 < a.cols) q += d3 * d3;
-    }
+    for (int k = 0; k < NV; k++) q += squares(shifted(v[k], shift, mean, chunk_at(k), a.cols));
     q = block_sum(q, cell);
     if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = make_float2(mean, q);
 }
@@ -258,6 +293,7 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
         b[k] = load_affine<T>(a.b, a.affine_f32, chunk_at(k), a.cols, 0.0f);
     }
     part += (int64_t)blockIdx.y * gridDim.x;
+    const RowShift shift((float)x[0]);
     const float n = (float)a.cols, inv = 1.0f / n;
     const auto count = [&](unsigned i) { return (float)min((int64_t)AZ_NORM_CHUNK, a.cols - (int64_t)i * AZ_NORM_CHUNK); };
     float s = 0.f, q = 0.f;
@@ -267,12 +303,13 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
         const float d = part[i].x - mean;
         q += part[i].y + count(i) * d * d;
     }
-    const float r = inv_sqrt(block_sum(q, cell) * inv + a.eps);
+    const float r = inv_sqrt(block_sum(q, cell) * inv * (shift.back() * shift.back()) + a.eps), rs = r * shift.back();
 #pragma unroll
-    for (int k = 0; k < NV; k++)
-        store4(y, chunk_at(k), a.cols, make_float4((v[k].x - mean) * r * w[k].x + b[k].x, (v[k].y - mean) * r * w[k].y + b[k].y,
-                                                   (v[k].z - mean) * r * w[k].z + b[k].z, (v[k].w - mean) * r * w[k].w + b[k].w));
-    if (a.mean && blockIdx.x == 0 && threadIdx.x == 0) { a.mean[blockIdx.y] = mean; a.rstd[blockIdx.y] = r; }
+    for (int k = 0; k < NV; k++) {
+        const float4 d = shifted(v[k], shift, mean, chunk_at(k), a.cols);
+        store4(y, chunk_at(k), a.cols, make_float4(d.x * rs * w[k].x + b[k].x, d.y * rs * w[k].y + b[k].y, d.z * rs * w[k].z + b[k].z, d.w * rs * w[k].w + b[k].w));
+    }
+    if (a.mean && blockIdx.x == 0 && threadIdx.x == 0) { a.mean[blockIdx.y] = shift.value(mean); a.rstd[blockIdx.y] = r; }
 }
 
 struct NormBwd {
@@ -288,7 +325,7 @@ struct NormBwd {
 // atomics, so the same call gives the same bits.  The threads of a workgroup that hold the same columns of different rows
 // add up through LDS at the end.
 // Elements past a row's end read as dy = 0 and have h = 0, so they add nothing to any sum, and they are not stored.  (Their h is
-// set and not left as -mean r: in a row without spread r is 1 / sqrt(eps), so that can overflow, and 0 times infinity is NaN.)
+// -mean times 0 and not times r: in a row without spread r is 1 / sqrt(eps), so that can overflow, and 0 times infinity is NaN.)
 // STREAM: x and dy, which this pass is the last to read, go past the L2 caches.
 // Without SUMS there is dx alone: a thread of a workgroup of 1024 has registers for 16 elements of x, dy and w, but not for
 // their sums too.
@@ -298,7 +335,7 @@ template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __laun
     __shared__ float cell[2][2][16];
     __shared__ float gather[GROUPS > 1 ? GROUPS * WIDTH : 1];
     const int t = threadIdx.x % TPR, cols = (int)a.cols, packs = cols / N, last = packs * N + t;
-    const bool full = packs == TPR * NV, tail = last < cols;
+    const bool tail = last < cols;
     const float inv = 1.0f / (float)cols;
     float w[NV][N], dw[SUMS ? NV : 1][N], db[SUMS ? NV : 1][N], dw1 = 0.f, db1 = 0.f;
 #pragma unroll
@@ -334,17 +371,13 @@ template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __laun
     int turn = 0;
     for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += step, row += step, turn ^= 1) {
         const float mean = next_mean, r = next_r;
-        const float h1 = tail ? ((float)next_x1 - mean) * r : 0.f;
+        const float h1 = ((float)next_x1 - mean) * (tail ? r : 0.f);
         float h[NV][N], g[NV][N], g1 = (float)next_dy1;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
+        for (int k = 0; k < NV; k++) {
+            const float rk = k * TPR + t < packs ? r : 0.f;
 #pragma unroll
-            for (int e = 0; e < N; e++) { h[k][e] = ((float)next_x[k][e] - mean) * r; g[k][e] = (float)next_dy[k][e]; }
-        if (!full) {
-#pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int e = 0; e < N; e++) h[k][e] = k * TPR + t < packs ? h[k][e] : 0.f;
+            for (int e = 0; e < N; e++) { h[k][e] = ((float)next_x[k][e] - mean) * rk; g[k][e] = (float)next_dy[k][e]; }
         }
         if (first + step < a.rows) ask(row + step);
         dw1 += g1 * h1;

@@ -81,6 +81,8 @@ template <int CTRL> __device__ __forceinline__ uint32_t dpp_row(uint32_t x)
 
 #define AZ_QUAD_XOR1 0xb1               // DPP quad_perm 1,0,3,2
 #define AZ_QUAD_XOR2 0x4e               // DPP quad_perm 2,3,0,1
+#define AZ_QUAD_FIRST 0x00              // DPP quad_perm 0,0,0,0
+#define AZ_ROW_LANE(n) (0x150 + (n))    // DPP row_newbcast: lane n of 16 in all of them
 #define AZ_ROW_HALF_MIRROR 0x141        // DPP row_half_mirror: lane i of eight takes lane 7 - i
 
 // Sums over 4 and 8 neighbouring lanes and over the 16 lanes of a DPP row, in every lane, the same bits in all of them (each step adds the same two partial

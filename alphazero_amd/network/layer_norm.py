@@ -16,8 +16,12 @@ from .device_ops import binding
 
 def _plain(x, weight, bias, eps):
     f = x.float()
-    centred = f - f.mean(-1, keepdim=True)
-    y = centred / torch.sqrt((centred * centred).mean(-1, keepdim=True) + eps)
+    # relative to the row's first value, as the kernels work (csrc/az_norm_kernels.h says why); the derivative is the same
+    first = f[..., :1].detach()
+    scale = torch.where(first.abs() < 2.0 ** 102, 1.0, 2.0 ** -30)
+    d = f * scale - first * scale
+    centred = d - d.mean(-1, keepdim=True)
+    y = centred / (torch.sqrt((centred * centred).mean(-1, keepdim=True) / (scale * scale) + eps) * scale)
     if weight is not None:
         y = y * weight.float()
     if bias is not None:
