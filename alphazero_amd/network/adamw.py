@@ -115,6 +115,9 @@ def _plain_step(p, g, m, v, step, lr, betas, eps, weight_decay, m_scale=None, v_
     p_.copy_(w - w * (lr * weight_decay) - new_m / denom * (lr / (1.0 - beta1 ** step)))
 
 
+_CONSTANTS = ("lr", "betas", "eps", "weight_decay")    # of a group (PyTorch adds to self.defaults when a state is set)
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW as a PyTorch optimizer.  state_bits=8 holds the state of every parameter of at least `min_8bit_size` elements in
     8 bits (biases and other small tensors stay in 32).  A checkpoint of either kind loads into the other.
@@ -195,7 +198,7 @@ class AdamW(torch.optim.Optimizer):
         """Takes the state of an AdamW with either kind of state (PyTorch's own among them) and converts it to this one's.
         Nothing is changed where that fails."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
-        if any("exp_avg" not in st or "exp_avg_sq" not in st for st in saved.values()) or any(k not in g for g in groups for k in self.defaults):
+        if any("exp_avg" not in st or "exp_avg_sq" not in st for st in saved.values()) or any(k not in g for g in groups for k in _CONSTANTS):
             raise ValueError("not the state of an AdamW optimizer")
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state of an optimizer with other parameter groups")
