@@ -116,6 +116,9 @@ def _plain_step(p, g, m, v, step, lr, betas, eps, weight_decay, m_scale=None, v_
 
 
 _CONSTANTS = ("lr", "betas", "eps", "weight_decay")    # of a group (PyTorch adds to self.defaults when a state is set)
+_STATE_KEYS = {"step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"}
+# what PyTorch's optimizers of this family keep in their groups beside the constants
+_TORCH_KEYS = {"amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay"}
 
 
 class AdamW(torch.optim.Optimizer):
@@ -195,20 +198,36 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """Takes the state of an AdamW with either kind of state (PyTorch's own among them) and converts it to this one's.
-        Nothing is changed where that fails."""
+        """Takes the state of an AdamW with either kind of state (PyTorch's own among them) and converts it to this one's.  The
+        states of other optimizers, and of PyTorch's with amsgrad, maximize or a weight decay that goes through the
+        gradient, are refused.  Nothing is changed where that fails."""
+        # as the last of the hooks before loading, so that the state is what the user's own made of it, and is there when
+        # those after loading run
+        hook = self.register_load_state_dict_pre_hook(AdamW._taken)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+
+    def _taken(self, state_dict):
         saved, groups = state_dict["state"], state_dict["param_groups"]
-        if any("exp_avg" not in st or "exp_avg_sq" not in st for st in saved.values()) or any(k not in g for g in groups for k in _CONSTANTS):
+        if any("exp_avg" not in st or "exp_avg_sq" not in st or set(st) - _STATE_KEYS for st in saved.values()) \
+                or any(k not in g for g in groups for k in _CONSTANTS):
             raise ValueError("not the state of an AdamW optimizer")
+        for g in groups:
+            theirs = _TORCH_KEYS & set(g)
+            if theirs and "amsgrad" not in g:
+                raise ValueError("the state of another optimizer than AdamW")     # of the same family, such as RAdam
+            if g.get("amsgrad") or g.get("maximize") or (not g.get("decoupled_weight_decay", True) and g["weight_decay"] != 0):
+                raise ValueError("this AdamW has no amsgrad, no maximize and no weight decay through the gradient")
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state of an optimizer with other parameter groups")
         ids = [i for g in groups for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
+        # PyTorch casts every state tensor that it finds by its number to its parameter's type, which codes and scales must not be;
+        # what stands under the parameter itself it takes as it is
         new = {p: self._converted(p, saved[i]) for i, p in zip(ids, params) if i in saved}
-        # PyTorch casts every state tensor to its parameter's type on loading, which codes and scales must not be: only the
-        # groups go that way
-        super().load_state_dict({"state": {}, "param_groups": groups})
-        self.state.update(new)
+        return {"state": new, "param_groups": [{k: v for k, v in g.items() if k not in _TORCH_KEYS} for g in groups]}
 
     def _converted(self, p, st):
         new = self._new_state(p)
