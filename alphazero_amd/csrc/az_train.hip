@@ -139,13 +139,16 @@ struct FwdType {
 
 // Workgroups of the backward pass, each of which leaves one row of partial sums: a function of the sizes alone, so the order
 // of the sums is the same on every call.  Four rows or more for each group of threads where there are rows enough, since
-// every workgroup costs a row of sums written and read again.
+// every workgroup costs a row of sums written and read again, but so many workgroups that no thread adds up more than 64 rows, or
+// rows / 1024 if that is more.  With the groups' sums and the workgroups' added to that, a float32 sum over the rows is
+// a chain of at most rows / 1024 + 96 additions in every form.
 int64_t bwd_parts(int64_t rows, int64_t cols, int32_t type)
 {
     if (rows <= 0) return 0;
-    if (norm_sums_apart(cols, type)) return std::min<int64_t>(rows, 64);
-    const int64_t packs = norm_packs(cols, type), groups = norm_groups(packs, type), each = (rows + groups - 1) / groups;
-    return std::min(norm_bwd_blocks(cols, type), std::max((each + 3) / 4, std::min<int64_t>(each, 64)));
+    const bool apart = norm_sums_apart(cols, type);
+    const int64_t packs = norm_packs(cols, type), groups = apart ? 1 : norm_groups(packs, type), each = (rows + groups - 1) / groups;
+    const int64_t parts = apart ? std::min<int64_t>(rows, 64) : std::min(norm_bwd_blocks(cols, type), std::max((each + 3) / 4, std::min<int64_t>(each, 64)));
+    return std::max(parts, std::min((each + 63) / 64, 1024 / groups));
 }
 
 struct BwdForm {
