@@ -9,7 +9,7 @@ import numpy as np
 import torch
 
 from ..engine import Engine, game_config_to_engine_kwargs
-from ..network.model import AZNet, fold_to_blob, random_net
+from ..network.model import AZNet, check_weights, fold_to_blob, random_net
 from ..processing.state_converter import StateTensorConverter, TensorActionConverter
 
 
@@ -102,6 +102,11 @@ class NNEvaluator:
         net = self._net     # (never written to again: _refold makes another one)
         return lambda planes: self._forward(net, planes)
 
+    def _take(self, state_dict):
+        check_weights(self.net, state_dict)     # (weights of another network are refused with nothing of them taken)
+        self.net.load_state_dict(state_dict)
+        self._refold()
+
     def load(self, filename):
         self.rwlock.w_acquire()
         try:
@@ -109,8 +114,7 @@ class NNEvaluator:
             # {'model', 'opt', 'global_step'} in '<prefix>-<step>'), which is how weights reach the evaluators in the
             # reference: net.save('.../ckpt') then nn_eval.load('.../ckpt-<step>') (train/parallel/evaluator.py:109)
             ck = torch.load(filename, weights_only=True, map_location="cpu")
-            self.net.load_state_dict(ck["model"] if "model" in ck else ck)
-            self._refold()
+            self._take(ck["model"] if "model" in ck else ck)
         finally:
             self.rwlock.w_release()
 
@@ -125,7 +129,6 @@ class NNEvaluator:
     def set_weights(self, state_dict):
         self.rwlock.w_acquire()
         try:
-            self.net.load_state_dict(state_dict)
-            self._refold()
+            self._take(state_dict)
         finally:
             self.rwlock.w_release()

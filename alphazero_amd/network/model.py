@@ -157,6 +157,16 @@ def fold_to_blob(net):
     return np.concatenate(parts).astype(np.float32)
 
 
+def check_weights(net, state):
+    """Raises what net.load_state_dict(state) would, before a single tensor has been copied."""
+    own = net.state_dict()
+    wrong = ["%s is missing" % k for k in own if k not in state] + ["%s is not of this network" % k for k in state if k not in own]
+    wrong += ["%s has shape %s, not %s" % (k, tuple(getattr(state[k], "shape", ())), tuple(t.shape)) for k, t in own.items()
+              if k in state and getattr(state[k], "shape", None) != t.shape]
+    if wrong:
+        raise RuntimeError("weights of another network: " + ", ".join(wrong[:5]) + (", and %d more" % (len(wrong) - 5) if len(wrong) > 5 else ""))
+
+
 def random_net(board_height, board_width, flat_move_output, num_blocks, channels=256, seed=0, perturb_bn=False, norm="batch"):
     """Seeded glorot-uniform network; perturb_bn randomises BN statistics so folding is exercised."""
     g = torch.Generator().manual_seed(seed)

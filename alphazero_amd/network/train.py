@@ -24,7 +24,7 @@ import torch.nn.functional as F
 import yaml
 
 from .adamw import AdamW
-from .model import AZNet, CenterBN
+from .model import AZNet, CenterBN, check_weights
 
 _DEFAULT_TRAIN_CONFIG = {
     "num_blocks": 19, "batch_decay": 0.9,
@@ -133,17 +133,21 @@ class Network:
 
     def load(self, filename):
         """A file of save(), or a bare state dict as NNEvaluator.save writes it (weights only: step and optimizer
-        state are then left as they are).  A file of another optimizer is refused (adamw and adamw8 take each other's)."""
+        state are then left as they are).  A file of another optimizer (adamw and adamw8 take each other's) or of another
+        network is refused, with nothing of it taken."""
         ck = torch.load(filename, weights_only=True, map_location=self.device)
         if "model" not in ck:
+            check_weights(self.net, ck)
             self.net.load_state_dict(ck)
             return
         of_adamw = "betas" in ck["opt"]["param_groups"][0]
         if of_adamw != isinstance(self.opt, AdamW):
             raise ValueError("%r holds the state of %s" % (filename, "an AdamW optimizer" if of_adamw else "a momentum optimizer"))
+        step = int(ck["global_step"])
+        check_weights(self.net, ck["model"])
+        self.opt.load_state_dict(ck["opt"])     # (an optimizer that refuses has changed nothing)
         self.net.load_state_dict(ck["model"])
-        self.opt.load_state_dict(ck["opt"])
-        self.global_step = int(ck["global_step"])
+        self.global_step = step
 
 
 def latest_checkpoint(save_dir):
