@@ -43,3 +43,20 @@ def test_build_compiles_what_is_already_there():
     finally:
         g.subprocess.check_call = real
     assert ran[0][0] == "make" and "-B" in ran[0]
+
+
+def test_the_c_library_needs_no_pytorch(tmp_path):
+    """With a Python that has no PyTorch, or without a Python, libazamd.so is all that is built, and nothing fails."""
+    bare = tmp_path / "python"
+    bare.write_text("#!/bin/sh\nexec %s -S -E \"$@\"\n" % shutil.which("python3"))
+    bare.chmod(0o755)
+    for python in (str(bare), str(tmp_path / "no-such-python")):
+        out = _would_run("-B", "PYTHON=" + python)
+        assert "-o libazamd.so" in out and "_train_ops" not in out
+    assert "-o ../network/_train_ops.so" in _would_run("-B")
+
+
+def test_another_pytorch_rebuilds_the_binding():
+    import torch
+    out = _would_run("-W", os.path.join(os.path.dirname(torch.__file__), "version.py"))
+    assert "az_torch.cpp -o ../network/_train_ops.so" in out
