@@ -5,7 +5,9 @@
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <string>
 #include <vector>
@@ -29,6 +31,13 @@ bool capturing(const at::Tensor &t)
     if (hipStreamIsCapturing(stream_of(t), &status) == hipSuccess) return status != hipStreamCaptureStatusNone;
     (void)hipGetLastError();   // (the default stream cannot be asked while another thread captures)
     return true;
+}
+
+// A tracer records PyTorch's own operations only: what is launched here would be missing from the graph, its result a constant.
+void not_traced(const char *what)
+{
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+        throw std::runtime_error(std::string(what) + " cannot be traced on the GPU");
 }
 
 void launched(int rc)
@@ -133,6 +142,7 @@ std::optional<at::Tensor> layer_norm(const at::Tensor &x, const std::optional<at
     if (weight && bias && weight->scalar_type() != bias->scalar_type()) type_error("weight and bias must have one type");
     if (x.is_cpu()) return std::nullopt;
     if (!x.is_cuda()) value_error("layer_norm runs on the GPU or the CPU, not on " + x.device().str());
+    not_traced("layer_norm");
     for (const at::Tensor *t : {&x, weight ? &*weight : nullptr, bias ? &*bias : nullptr})
         if (t && t->_fw_grad(0).defined()) throw std::runtime_error("layer_norm has no forward-mode derivative on the GPU");
     const bool record = at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad()));
@@ -210,6 +220,7 @@ int adamw_step(const py::sequence &params_, const py::sequence &grads_, const py
     }
     if (device.is_cpu()) return 1;
     if (!there) value_error("adamw_step runs on the GPU or the CPU, not on " + device.str());
+    not_traced("an AdamW step");
     if (capturing(params[0])) throw std::runtime_error("an AdamW step cannot be captured into a HIP graph: every replay would be the same step");
     int rc;
     {
@@ -237,6 +248,7 @@ std::optional<at::Tensor> dequantize_state(const at::Tensor &codes, const at::Te
         value_error(std::to_string(n) + " codes need dense memory and " + std::to_string(blocks) + " scales, not " + std::to_string(scales.numel()));
     if (codes.is_cpu()) return std::nullopt;
     if (!codes.is_cuda()) value_error("dequantize_state runs on the GPU or the CPU, not on " + codes.device().str());
+    not_traced("dequantize_state");
     at::Tensor out = at::empty_strided(codes.sizes(), codes.strides(), codes.options().dtype(at::kFloat));
     launched(az_dequantize_state_dev(codes.get_device(), stream_of(codes), codes.const_data_ptr(), static_cast<const float *>(scales.const_data_ptr()), n,
                                      type == at::kChar, static_cast<float *>(out.data_ptr())));

@@ -33,7 +33,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm of x (float32, bfloat16 or float16; any leading axes, any strides) over its last axis.  weight and bias have
     that axis' length and are both float32 or both of x's type; either may be None.  The result is contiguous and of x's type;
     statistics and the sums of the gradients are float32 and rounded once.  Differentiable once in x, weight and bias.
-    A forward without gradients can be captured into a HIP graph; one that records gradients cannot."""
+    A forward without gradients can be captured into a HIP graph; one that records gradients cannot.  Tracers
+    (torch.jit.trace, make_fx) do not see inside it: on the GPU it refuses to be traced."""
     y = binding().layer_norm(x, weight, bias, eps)
     return y if y is not None else _plain(x, weight, bias, eps)
 
