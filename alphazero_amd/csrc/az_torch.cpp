@@ -47,8 +47,9 @@ void launched(int rc)
 
 // ---- layer norm -----------------------------------------------------------------------------------------------------------
 // x as rows of `cols` neighbouring elements, and the elements from one row to the next; copied only if it is not one
-std::pair<at::Tensor, int64_t> as_rows(const at::Tensor &x, int64_t cols)
+std::pair<at::Tensor, int64_t> as_rows(const at::Tensor &x_, int64_t cols)
 {
+    const at::Tensor x = x_.is_neg() ? x_.resolve_neg() : x_;     // (a sign that is not in memory yet)
     if (x.is_contiguous()) return {x, cols};
     if (x.dim() > 1 && (x.stride(-1) == 1 || cols == 1)) {
         int64_t step = -1, next = 0;   // of the leading axes, from the last one: the stride that continues the ones so far
@@ -64,13 +65,16 @@ std::pair<at::Tensor, int64_t> as_rows(const at::Tensor &x, int64_t cols)
     return {x.contiguous(), cols};
 }
 
+// a weight or bias as its elements lie in memory
+at::Tensor plain(const at::Tensor &t) { return !t.defined() ? t : t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
+
 const void *pointer(const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
 at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias, double eps, float *mean, float *rstd)
 {
     const int64_t cols = x.size(-1), rows = x.numel() / cols;
     const auto [v, stride] = as_rows(x, cols);
-    const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+    const at::Tensor w = plain(weight), b = plain(bias);
     const at::ScalarType affine = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
     const int32_t type = type_id(x.scalar_type());
     at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), space;
@@ -101,7 +105,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm can be differentiated once only");
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &stats = saved[2];
-        const at::Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
+        const at::Tensor w = plain(saved[1]);
         const int64_t cols = x.size(-1), rows = x.numel() / cols;
         const auto affine = (at::ScalarType)ctx->saved_data["affine"].toInt();
         const auto [v, x_stride] = as_rows(x, cols);
@@ -175,8 +179,9 @@ int adamw_step(const py::sequence &params_, const py::sequence &grads_, const py
     if (step < 1) value_error("steps are counted from 1");
     if (m_scales_.has_value() != v_scales_.has_value()) value_error("8-bit states need the scales of both");
     const bool eight = m_scales_.has_value();
-    const auto params = tensors_of(params_, "a parameter"), grads = tensors_of(grads_, "a gradient"), m = tensors_of(m_, "exp_avg"), v = tensors_of(v_, "exp_avg_sq");
+    const auto params = tensors_of(params_, "a parameter"), m = tensors_of(m_, "exp_avg"), v = tensors_of(v_, "exp_avg_sq");
     const auto ms = eight ? tensors_of(*m_scales_, "a scale") : std::vector<at::Tensor>(), vs = eight ? tensors_of(*v_scales_, "a scale") : std::vector<at::Tensor>();
+    auto grads = tensors_of(grads_, "a gradient");
     const size_t n = params.size();
     if (grads.size() != n || m.size() != n || v.size() != n || (eight && (ms.size() != n || vs.size() != n)))
         value_error("one gradient, two states and their scales for every parameter");
@@ -188,12 +193,13 @@ int adamw_step(const py::sequence &params_, const py::sequence &grads_, const py
     std::vector<void *> pp(n), mp(n), vp(n);
     std::vector<const void *> gp(n);
     std::vector<float *> msp(eight ? n : 0), vsp(eight ? n : 0);
+    const bool there = device.is_cuda();
     const auto check = [&](const at::Tensor &t, at::ScalarType kind, const char *what) {
         if (t.layout() != at::kStrided) type_error(std::string(what) + " is not a strided tensor");
         if (t.scalar_type() != kind) type_error(std::string(what) + " is not " + name_of(kind));
         if (t.device() != device) value_error(std::string(what) + " is not on " + device.str());
+        if (there && t.is_neg()) type_error(std::string(what) + " is negated in name only: resolve_neg() it");
     };
-    const bool there = device.is_cuda();
     for (size_t i = 0; i < n; i++) {
         const at::Tensor &p = params[i];
         check(p, type, "a parameter");
@@ -203,6 +209,7 @@ int adamw_step(const py::sequence &params_, const py::sequence &grads_, const py
             if (!(p.is_contiguous() && t.is_contiguous()) && !(p.is_non_overlapping_and_dense() && p.strides() == t.strides()))
                 value_error(std::string(what) + " does not lie in memory as its parameter does (or the parameter is not dense)");
         };
+        if (there && grads[i].is_neg()) grads[i] = grads[i].resolve_neg();      // (read only: a copy does)
         alike(grads[i], type, "gradient");
         alike(m[i], eight ? at::kChar : at::kFloat, "exp_avg");
         alike(v[i], eight ? at::kByte : at::kFloat, "exp_avg_sq");
@@ -248,6 +255,7 @@ std::optional<at::Tensor> dequantize_state(const at::Tensor &codes, const at::Te
         value_error(std::to_string(n) + " codes need dense memory and " + std::to_string(blocks) + " scales, not " + std::to_string(scales.numel()));
     if (codes.is_cpu()) return std::nullopt;
     if (!codes.is_cuda()) value_error("dequantize_state runs on the GPU or the CPU, not on " + codes.device().str());
+    if (scales.is_neg()) type_error("scales are negated in name only: resolve_neg() them");
     not_traced("dequantize_state");
     at::Tensor out = at::empty_strided(codes.sizes(), codes.strides(), codes.options().dtype(at::kFloat));
     launched(az_dequantize_state_dev(codes.get_device(), stream_of(codes), codes.const_data_ptr(), static_cast<const float *>(scales.const_data_ptr()), n,
