@@ -9,7 +9,7 @@ import numpy as np
 import torch
 
 from ..engine import Engine, game_config_to_engine_kwargs
-from ..network.model import AZNet, check_weights, fold_to_blob, random_net
+from ..network.model import AZNet, check_weights, fold_to_blob, norm_of, random_net
 from ..processing.state_converter import StateTensorConverter, TensorActionConverter
 
 
@@ -55,7 +55,7 @@ class NNEvaluator:
         self._H, self._W, self._O = kw["board_height"], kw["board_width"], game_config['flat_move_output']
         self.net = net if net is not None else random_net(self._H, self._W, self._O, num_blocks, channels, seed=seed, norm=norm)
         self.rwlock = RWLock()
-        if self.net.norm == "batch":
+        if norm_of(self.net) == "batch":
             self._eng = Engine(n_slots=max_batch_size, num_blocks=num_blocks, channels=channels, tower_dtype=dtype, device=device, **kw)
         else:
             self._eng, self._device = None, torch.device("cuda", device)

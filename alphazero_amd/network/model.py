@@ -77,6 +77,11 @@ def _glorot_linear(lin):
     nn.init.zeros_(lin.bias)
 
 
+def norm_of(net):
+    """'batch' or 'layer'; a network that does not say has batch norm."""
+    return getattr(net, "norm", "batch")
+
+
 class AZNet(nn.Module):
     def __init__(self, board_height, board_width, flat_move_output, num_blocks, channels=256, planes=17, norm="batch"):
         super().__init__()
@@ -110,7 +115,7 @@ class AZNet(nn.Module):
             self.to(memory_format=torch.channels_last)
 
     def forward(self, x):
-        if self.norm == "layer":
+        if norm_of(self) == "layer":
             x = x.contiguous(memory_format=torch.channels_last)
         r = F.relu(self.stem_bn(self.stem(x)))
         for i in range(self.NB):
@@ -136,7 +141,7 @@ def _fold(conv, bn):
 
 def fold_to_blob(net):
     """BN-folded float32 weight blob in the layout az_tower_load_weights expects."""
-    if net.norm != "batch":
+    if norm_of(net) != "batch":
         raise ValueError("a network with layer norm cannot be folded into the tower's weights")
     parts = []
 

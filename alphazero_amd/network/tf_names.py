@@ -18,6 +18,8 @@ unpinned against a real checkpoint.
 import numpy as np
 import torch
 
+from .model import norm_of
+
 
 def _bn_items(prefix, bn):
     return [(prefix + "/BatchNorm/beta", bn.beta), (prefix + "/BatchNorm/moving_mean", bn.running_mean),
@@ -26,7 +28,7 @@ def _bn_items(prefix, bn):
 
 def _entries(net):
     """[(tf_name, tensor, kind)] in graph construction order; kind: conv | linear_w | vec."""
-    if net.norm != "batch":
+    if norm_of(net) != "batch":
         raise ValueError("the reference's graph has batch norm: a network with layer norm has no names in it")
     out = [("model/W0", net.stem.weight, "conv")]
     out += [(n, t, "vec") for n, t in _bn_items("model/bn", net.stem_bn)]
