@@ -317,12 +317,14 @@ struct NormBwd {
     const float *mean, *rstd;
     void *dx;                // null: not wanted
     float *part;             // [2][parts][cols] sums of the workgroups' rows: dw, then db; null: not wanted
+    int64_t parts, turns, times;   // a workgroup writes its sums after so many turns, so many times in all
     int64_t rows, cols, dy_stride, x_stride, dx_stride;
     bool affine_f32, stream; // stream: dx is larger than the L2 caches
 };
 
 // dx of the rows, and for every workgroup the sums of dy * h and dy over its rows in the order in which it meets them: no
-// atomics, so the same call gives the same bits.  The threads of a workgroup that hold the same columns of different rows
+// atomics, so the same call gives the same bits.  (A workgroup of one group writes them out after a number of rows and starts
+// anew: a long chain of additions would lose what a short one keeps.)  The threads of a workgroup that hold the same columns of different rows
 // add up through LDS at the end.
 // Elements past a row's end read as dy = 0 and have h = 0, so they add nothing to any sum, and they are not stored.  (Their h is
 // -mean times 0 and not times r: in a row without spread r is 1 / sqrt(eps), so that can overflow, and 0 times infinity is NaN.)
@@ -367,6 +369,26 @@ template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __laun
         next_mean = i < a.rows ? a.mean[i] : 0.f;
         next_r = i < a.rows ? a.rstd[i] : 0.f;
     };
+    // one partial row of a workgroup that is a single group; its sums start anew
+    int64_t left = a.turns, written = 0;
+    const auto write = [&] {
+        float *to = a.part + (written++ * gridDim.x + blockIdx.x) * a.cols;
+#pragma unroll
+        for (int k = 0; k < (SUMS ? NV : 0); k++) {
+            const int at = (k * TPR + t) * N;
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                if (k * TPR + t < packs) {
+                    store4(to + at + e, make_float4(dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]));
+                    store4(to + a.parts * a.cols + at + e, make_float4(db[k][e], db[k][e + 1], db[k][e + 2], db[k][e + 3]));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < N; e++) dw[k][e] = db[k][e] = 0.f;
+        }
+        if (tail) { to[last] = dw1; to[a.parts * a.cols + last] = db1; }
+        dw1 = db1 = 0.f;
+    };
     ask(row);
     int turn = 0;
     for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += step, row += step, turn ^= 1) {
@@ -396,6 +418,8 @@ template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __laun
                 s[0] += g[k][e];
                 s[1] += g[k][e] * h[k][e];
             }
+        if constexpr (SUMS && GROUPS == 1)
+            if (a.part && --left == 0) { write(); left = a.turns; }
         if (!a.dx) continue;
         group_sum<TPR>(s, cell, turn);
         const float m0 = s[0] * inv, m1 = s[1] * inv;
@@ -411,27 +435,19 @@ template <typename T, int TPR, int NV, bool STREAM, bool SUMS> __global__ __laun
         }
     }
     if (!a.part) return;
+    if constexpr (SUMS && GROUPS == 1) {
+        while (written < a.times) write();       // (zeros where this workgroup had a row less than others)
+    } else if constexpr (SUMS) {
 #pragma unroll
-    for (int which = 0; which < (SUMS ? 2 : 0); which++) {
-        float *part = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.cols;
-        if constexpr (GROUPS == 1) {
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const float *f = which ? db[SUMS ? k : 0] : dw[SUMS ? k : 0];
-                if (k * TPR + t < packs) {
-#pragma unroll
-                    for (int e = 0; e < N; e += 4) store4(part + (k * TPR + t) * N + e, make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]));
-                }
-            }
-            if (tail) part[last] = which ? db1 : dw1;
-        } else {
+        for (int which = 0; which < 2; which++) {
+            float *part = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.cols;
             __syncthreads();
             float *mine = gather + (threadIdx.x / TPR) * WIDTH;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 if (k * TPR + t < packs) {
 #pragma unroll
-                    for (int e = 0; e < N; e++) mine[(k * TPR + t) * N + e] = which ? db[SUMS ? k : 0][e] : dw[SUMS ? k : 0][e];
+                    for (int e = 0; e < N; e++) mine[(k * TPR + t) * N + e] = which ? db[k][e] : dw[k][e];
                 }
             }
             if (tail) mine[last] = which ? db1 : dw1;

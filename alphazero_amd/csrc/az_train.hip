@@ -137,22 +137,33 @@ struct FwdType {
     }
 };
 
-// Workgroups of the backward pass, each of which leaves one row of partial sums: a function of the sizes alone, so the order
-// of the sums is the same on every call.  Four rows or more for each group of threads where there are rows enough, since
-// every workgroup costs a row of sums written and read again, but so many workgroups that no thread adds up more than 64 rows, or
-// rows / 1024 if that is more.  With the groups' sums and the workgroups' added to that, a float32 sum over the rows is
-// a chain of at most rows / 1024 + 96 additions in every form.
-int64_t bwd_parts(int64_t rows, int64_t cols, int32_t type)
-{
-    if (rows <= 0) return 0;
-    const bool apart = norm_sums_apart(cols, type);
-    const int64_t packs = norm_packs(cols, type), groups = apart ? 1 : norm_groups(packs, type), each = (rows + groups - 1) / groups;
-    const int64_t parts = apart ? std::min<int64_t>(rows, 64) : std::min(norm_bwd_blocks(cols, type), std::max((each + 3) / 4, std::min<int64_t>(each, 64)));
-    return std::max(parts, std::min((each + 63) / 64, 1024 / groups));
-}
+// Workgroups of the backward pass and how many rows of partial sums each of them leaves: functions of the sizes alone, so the
+// order of the sums is the same on every call.  Four rows or more for each group of threads where there are rows enough,
+// since every partial row is written and read again, but so many partial rows that no thread adds up more than 64 rows, or
+// rows / 1024 if that is more.  With the groups' sums and the partial rows' added to that, a float32 sum over the rows is a
+// chain of at most rows / 1024 + 96 additions in every form.
+// (Several partial rows to a workgroup cost less than more workgroups: 40 000 rows of 8192 bfloat16 361 us and 414, 344
+// with a chain of 157.)
+struct BwdParts {
+    int64_t blocks = 0, turns = 0, times = 1;     // a workgroup writes its sums after so many turns, so many times
+    int64_t parts() const { return blocks * times; }
+    BwdParts(int64_t rows, int64_t cols, int32_t type)
+    {
+        if (rows <= 0) return;
+        const int64_t longest = std::max<int64_t>(64, (rows + 1023) / 1024);
+        if (norm_sums_apart(cols, type)) { blocks = std::max(std::min<int64_t>(rows, 64), (rows + longest - 1) / longest); return; }
+        const int64_t packs = norm_packs(cols, type), groups = norm_groups(packs, type), each = (rows + groups - 1) / groups;
+        blocks = std::min(norm_bwd_blocks(cols, type), std::max((each + 3) / 4, std::min<int64_t>(each, 64)));
+        turns = (each + blocks - 1) / blocks;
+        if (groups > 1) return;      // (with several groups to a workgroup 1024 of them or more in all)
+        times = (turns + longest - 1) / longest;
+        turns = longest;
+    }
+};
+int64_t bwd_parts(int64_t rows, int64_t cols, int32_t type) { return BwdParts(rows, cols, type).parts(); }
 
 struct BwdForm {
-    const NormBwd &a; hipStream_t st; int64_t parts;
+    const NormBwd &a; hipStream_t st; int64_t grid;
     template <typename T, int TPR, int NV> void operator()() const
     {
         if constexpr (TPR * NV * Pack<T>::N > 8192) {
@@ -160,15 +171,15 @@ struct BwdForm {
             if (!a.dx) return;
             if (a.stream) k_layer_norm_bwd<T, TPR, NV, true, false><<<blocks, norm_threads(TPR), 0, st>>>(a);
             else k_layer_norm_bwd<T, TPR, NV, false, false><<<blocks, norm_threads(TPR), 0, st>>>(a);
-        } else if (a.stream) k_layer_norm_bwd<T, TPR, NV, true, true><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
-        else k_layer_norm_bwd<T, TPR, NV, false, true><<<(unsigned)parts, norm_threads(TPR), 0, st>>>(a);
+        } else if (a.stream) k_layer_norm_bwd<T, TPR, NV, true, true><<<(unsigned)grid, norm_threads(TPR), 0, st>>>(a);
+        else k_layer_norm_bwd<T, TPR, NV, false, true><<<(unsigned)grid, norm_threads(TPR), 0, st>>>(a);
     }
 };
 struct BwdType {
     const NormBwd &a; float2 *part; void *dw, *db; hipStream_t st; int32_t type;
     template <typename T> void operator()() const
     {
-        const int64_t parts = bwd_parts(a.rows, a.cols, type);
+        const int64_t parts = a.parts;
         if (parts > 0) {
             const int64_t chunks = norm_chunks(a.rows, a.cols, type);
             // (the pass for dx comes after it: it is the last to read x and dy and may take them past the caches; 4096 rows of 16384
@@ -176,7 +187,7 @@ struct BwdType {
             if (a.part && norm_sums_apart(a.cols, type))
                 k_layer_norm_cols_wide<T><<<dim3((unsigned)((a.cols + 1023) / 1024), (unsigned)parts), AZ_NORM_COLS_WIDE_THREADS, 0, st>>>(a);
             if (!norm_wide(a.cols, type)) {
-                norm_form<T>(norm_packs(a.cols, type), BwdForm{a, st, parts});
+                norm_form<T>(norm_packs(a.cols, type), BwdForm{a, st, BwdParts(a.rows, a.cols, type).blocks});
             } else if (a.dx && chunks) {
                 const dim3 grid((unsigned)chunks, (unsigned)a.rows);
                 k_layer_norm_chunk_sums<T><<<grid, AZ_NORM_WIDE_THREADS, 0, st>>>(a, part);
@@ -248,7 +259,8 @@ extern "C" int az_layer_norm_bwd_dev(int32_t device, void *stream, int32_t type,
     if (!dx && !sums) return AZ_OK;
     DeviceScope scope(device);
     if (scope.error != hipSuccess) return fail_hip("layer norm backward: device", scope.error);
-    const NormBwd a{dy, x, weight, mean, rstd, dx, sums && need ? workspace + chunk_floats : nullptr, rows, cols, dy_stride, x_stride, dx_stride,
+    const BwdParts plan(rows, cols, type);
+    const NormBwd a{dy, x, weight, mean, rstd, dx, sums && need ? workspace + chunk_floats : nullptr, plan.parts(), plan.turns, plan.times, rows, cols, dy_stride, x_stride, dx_stride,
                     affine_type == AZ_TYPE_F32, rows * cols * (type == AZ_TYPE_F32 ? 4 : 2) > AZ_L2_BYTES};
     by_type(type, BwdType{a, reinterpret_cast<float2 *>(workspace), dweight, dbias, static_cast<hipStream_t>(stream), type});
     const hipError_t e = hipGetLastError();
