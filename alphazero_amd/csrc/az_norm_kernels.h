@@ -69,13 +69,6 @@ template <int TPR, int N> __device__ __forceinline__ void group_sum(float (&v)[N
     }
 }
 
-// s / n to half a step
-__device__ __forceinline__ float mean_of(float s, float n, float inv)
-{
-    const float q = s * inv;
-    return fmaf(fmaf(-q, n, s), inv, q);
-}
-
 // 1 / sqrt(t) to one step of float32; the instruction takes no subnormal numbers
 __device__ __forceinline__ float inv_sqrt(float t) { return t < 0x1p-126f ? 1.0f / sqrtf(t) : __builtin_amdgcn_rsqf(t); }
 
@@ -88,6 +81,10 @@ struct RowShift {
     __device__ __forceinline__ explicit RowShift(float x0) : scale(fabsf(x0) < 0x1p102f ? 1.0f : 0x1p-30f), first(x0 * scale) {}
     __device__ __forceinline__ float operator()(float x) const { return fmaf(x, scale, -first); }
     __device__ __forceinline__ float back() const { return scale == 1.0f ? 1.0f : 0x1p30f; }
+    __device__ __forceinline__ float rstd(float squares, float inv, float eps) const     // from the sum of the squares of n d's, inv = 1 / n
+    {
+        return inv_sqrt(fmaf(squares, scale == 1.0f ? inv : inv * 0x1p60f, eps));
+    }
     __device__ __forceinline__ float value(float d) const { return fmaf(d, back(), first * back()); }   // the x whose d this is
 };
 
@@ -100,7 +97,8 @@ template <int TPR> __device__ __forceinline__ float first_lane(float x)
 {
     const uint32_t u = __float_as_uint(x);
     if constexpr (TPR == 4) return __uint_as_float(dpp_row<AZ_QUAD_FIRST>(u));
-    else if constexpr (TPR == 8) return __uint_as_float((threadIdx.x & 8) ? dpp_row<AZ_ROW_LANE(8)>(u) : dpp_row<AZ_ROW_LANE(0)>(u));
+    else if constexpr (TPR == 8)      // lane 0's in all 16, then lane 8's in the upper two banks of four
+        return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)dpp_row<AZ_ROW_LANE(0)>(u), (int)u, AZ_ROW_LANE(8), 0xf, 0xc, false));
     else if constexpr (TPR == 16) return __uint_as_float(dpp_row<AZ_ROW_LANE(0)>(u));
     else if constexpr (TPR == 32) {
         const uint32_t first = dpp_row<AZ_ROW_LANE(0)>(u);
@@ -123,7 +121,7 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads
     __shared__ float cell[2][1][16];
     const int t = threadIdx.x % TPR, cols = (int)a.cols, packs = cols / N, last = packs * N + t;
     const bool tail = last < cols;
-    const float n = (float)cols, inv = 1.0f / n;
+    const float inv = 1.0f / (float)cols;
     float w[NV][N], b[NV][N];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
@@ -168,7 +166,7 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads
 #pragma unroll
             for (int e = 0; e < N; e += 4) s[0] += (v[k][e] + v[k][e + 1]) + (v[k][e + 2] + v[k][e + 3]);
         group_sum<TPR>(s, cell, 0);
-        const float mean = mean_of(s[0], n, inv);     // of the row's values less its first
+        const float mean = s[0] * inv;     // of the row's values less its first
         v1 = tail ? v1 - mean : 0.f;
         q[0] = v1 * v1;
 #pragma unroll
@@ -183,7 +181,7 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(norm_threads
             for (int e = 0; e < N; e += 4)
                 q[0] += (v[k][e] * v[k][e] + v[k][e + 1] * v[k][e + 1]) + (v[k][e + 2] * v[k][e + 2] + v[k][e + 3] * v[k][e + 3]);
         group_sum<TPR>(q, cell, 1);
-        const float r = inv_sqrt(q[0] * inv * (shift.back() * shift.back()) + a.eps), rs = r * shift.back();
+        const float r = shift.rstd(q[0], inv, a.eps), rs = r * shift.back();
         if (row < a.rows) {
             T *y = static_cast<T *>(a.y) + row * a.y_stride;
 #pragma unroll
@@ -238,9 +236,9 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
         const RowShift shift((float)x[0]);
         float s = 0.f, q = 0.f;
         for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) s += sum4(shifted(x, shift, 0.f, c, a.cols));
-        const float mean = mean_of(block_sum(s, cell), (float)a.cols, inv);
+        const float mean = block_sum(s, cell) * inv;
         for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) q += squares(shifted(x, shift, mean, c, a.cols));
-        const float r = inv_sqrt(block_sum(q, cell) * inv * (shift.back() * shift.back()) + a.eps), rs = r * shift.back();
+        const float r = shift.rstd(block_sum(q, cell), inv, a.eps), rs = r * shift.back();
         for (int64_t c = threadIdx.x * 4; c < a.cols; c += step) {
             const float4 v = shifted(x, shift, mean, c, a.cols), w = load_affine<T>(a.w, a.affine_f32, c, a.cols, 1.0f);
             const float4 b = load_affine<T>(a.b, a.affine_f32, c, a.cols, 0.0f);
@@ -272,7 +270,7 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
     for (int k = 0; k < NV; k++) v[k] = load4(x, chunk_at(k), a.cols);
 #pragma unroll
     for (int k = 0; k < NV; k++) s += sum4(shifted(v[k], shift, 0.f, chunk_at(k), a.cols));
-    const float mean = mean_of(block_sum(s, cell), n, 1.0f / n);
+    const float mean = block_sum(s, cell) / n;
 #pragma unroll
     for (int k = 0; k < NV; k++) q += squares(shifted(v[k], shift, mean, chunk_at(k), a.cols));
     q = block_sum(q, cell);
@@ -294,16 +292,16 @@ template <typename T> __global__ __launch_bounds__(AZ_NORM_WIDE_THREADS) void k_
     }
     part += (int64_t)blockIdx.y * gridDim.x;
     const RowShift shift((float)x[0]);
-    const float n = (float)a.cols, inv = 1.0f / n;
+    const float inv = 1.0f / (float)a.cols;
     const auto count = [&](unsigned i) { return (float)min((int64_t)AZ_NORM_CHUNK, a.cols - (int64_t)i * AZ_NORM_CHUNK); };
     float s = 0.f, q = 0.f;
     for (unsigned i = threadIdx.x; i < gridDim.x; i += AZ_NORM_WIDE_THREADS) s += count(i) * part[i].x;
-    const float mean = mean_of(block_sum(s, cell), n, inv);
+    const float mean = block_sum(s, cell) * inv;
     for (unsigned i = threadIdx.x; i < gridDim.x; i += AZ_NORM_WIDE_THREADS) {
         const float d = part[i].x - mean;
         q += part[i].y + count(i) * d * d;
     }
-    const float r = inv_sqrt(block_sum(q, cell) * inv * (shift.back() * shift.back()) + a.eps), rs = r * shift.back();
+    const float r = shift.rstd(block_sum(q, cell), inv, a.eps), rs = r * shift.back();
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const float4 d = shifted(v[k], shift, mean, chunk_at(k), a.cols);
