@@ -42,8 +42,8 @@ bool norm_wide(int64_t cols, int32_t type) { return norm_packs(cols, type) > (ty
 bool norm_sums_apart(int64_t cols, int32_t type) { return norm_packs(cols, type) > (type == AZ_TYPE_F32 ? 2048 : 1024); }
 
 // Threads per row and packs per thread: the narrowest form that holds the row, one wave up to 256 packs.  (At least as many
-// threads as there can be elements past the last whole pack.)  Forward, 1 M rows: 8 float32 columns 14 us with four threads to
-// a row and 36 with sixteen, 32 bfloat16 columns 27 us with eight and 48 with sixteen.
+// threads as there can be elements past the last whole pack.)  Forward, 1 M rows: 8 float32 columns 15 us with four threads to
+// a row and 40 with sixteen, 32 bfloat16 columns 31 us with eight and 54 with sixteen.
 template <typename T, typename Launch> void norm_form(int64_t packs, const Launch &launch)
 {
     constexpr int NV = sizeof(T) == 4 ? 2 : 1;   // packs of 8 elements
@@ -74,10 +74,10 @@ int64_t norm_block(int64_t packs, int32_t type)
 }
 
 // Workgroups of a pass over many rows, each of which walks over its share of them.  More than the memory needs in flight only
-// spread the accesses: rows of 256 float32 (whole cache lines) take 65 us with 1024 workgroups forward and 71 with 2048
-// (185 k rows), 100 us backward with 768 and 107 with 1024.  Rows that end inside a line wait for each other's lines and want
-// more: 361 16-bit columns, 100 k rows: 34 us with 2048 and 38 with 1024; backward 43 with 1024 and 48 with 768.  Forms with a
-// workgroup to a row wait at its barriers and want all that fit (1500 16-bit columns: 32 us with 1024, 47 with 512).
+// spread the accesses: rows of 256 float32 (whole cache lines) take 65 us with 1024 workgroups forward and 74 with 2048
+// (185 k rows), 94 us backward with 768 and 96 with 1024.  Rows that end inside a line wait for each other's lines and want
+// more: 361 16-bit columns, 100 k rows: 27 us with 2048 and 29 with 1024; backward 48 with 1024 and 53 with 768.  Forms with a
+// workgroup to a row wait at its barriers and want all that fit (30 k rows of 2500 16-bit columns: 62 us with 1024, 77 with 512).
 bool norm_lines(int64_t cols, int32_t type) { return cols * (type == AZ_TYPE_F32 ? 4 : 2) % 128 == 0; }
 
 int64_t norm_fwd_blocks(int64_t cols, int32_t type)
@@ -98,8 +98,9 @@ int64_t norm_bwd_blocks(int64_t cols, int32_t type)
     return packs <= 512 ? 512 : 256;
 }
 
-// Of the eight L2 caches together.  What is larger is written, and read for the last time, past them: 361 16-bit columns, 100 k
-// rows, backward 43 us against 46; 256 float32 columns, 92 k rows, forward 32 against 36.
+// Of the eight L2 caches together.  What is larger is written, and read for the last time, past them: 256 float32 columns, 185 k
+// rows, backward 94 us against 106; 4096 rows of 16384 bfloat16, backward 150 against 157.  (In some sizes it is the other way
+// round, by less: 361 16-bit columns, 100 k rows, 48 us against 47; 1500 float32 columns, 100 k rows, 384 against 367.)
 #define AZ_L2_BYTES (32 << 20)
 
 template <typename Launch> void by_type(int32_t type, const Launch &launch)
@@ -183,7 +184,7 @@ struct BwdType {
         if (parts > 0) {
             const int64_t chunks = norm_chunks(a.rows, a.cols, type);
             // (the pass for dx comes after it: it is the last to read x and dy and may take them past the caches; 4096 rows of 16384
-            // bfloat16 200 us, the other way round 205, and 209 with dx first but through the caches)
+            // bfloat16 with the forward pass 200 us, the other way round 205, and 209 with dx first but through the caches)
             if (a.part && norm_sums_apart(a.cols, type))
                 k_layer_norm_cols_wide<T><<<dim3((unsigned)((a.cols + 1023) / 1024), (unsigned)parts), AZ_NORM_COLS_WIDE_THREADS, 0, st>>>(a);
             if (!norm_wide(a.cols, type)) {

@@ -342,7 +342,7 @@ int az_tower_leaf_compaction(az_engine *h, int32_t on);
 #define AZ_TYPE_F16 2
 /* Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias for `rows` rows of `cols` elements; row i of x
  * starts at element i * x_stride (0: the same row throughout).  weight / bias may be NULL (1 / 0) and are of affine_type, float32 or
- * x's type.  mean / rstd (float32, [rows]): what the backward pass needs, or both NULL.  workspace: 8-byte aligned,
+ * x's type.  mean / rstd (float32, [rows], each rounded once): what the backward pass needs, or both NULL.  workspace: 8-byte aligned,
  * az_layer_norm_fwd_workspace(type, rows, cols) floats (0 but for a few very wide rows); a workspace may be reused as soon as the
  * stream has passed the call. */
 int64_t az_layer_norm_fwd_workspace(int32_t type, int64_t rows, int64_t cols);
