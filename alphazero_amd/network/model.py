@@ -166,8 +166,9 @@ def check_weights(net, state):
     """Raises what net.load_state_dict(state) would, before a single tensor has been copied."""
     own = net.state_dict()
     wrong = ["%s is missing" % k for k in own if k not in state] + ["%s is not of this network" % k for k in state if k not in own]
-    wrong += ["%s has shape %s, not %s" % (k, tuple(getattr(state[k], "shape", ())), tuple(t.shape)) for k, t in own.items()
-              if k in state and getattr(state[k], "shape", None) != t.shape]
+    wrong += ["%s is no tensor" % k for k in own if k in state and not torch.is_tensor(state[k])]
+    wrong += ["%s has shape %s, not %s" % (k, tuple(state[k].shape), tuple(t.shape)) for k, t in own.items()
+              if torch.is_tensor(state.get(k)) and state[k].shape != t.shape]
     if wrong:
         raise RuntimeError("weights of another network: " + ", ".join(wrong[:5]) + (", and %d more" % (len(wrong) - 5) if len(wrong) > 5 else ""))
 

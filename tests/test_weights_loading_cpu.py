@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from alphazero_amd.evaluator import nn_eval
-from alphazero_amd.network.model import random_net
+from alphazero_amd.network.model import check_weights, random_net
 from alphazero_amd.network.train import Network
 
 CFG = {"board_height": 3, "board_width": 3, "flat_move_output": 9}
@@ -108,3 +108,12 @@ def test_evaluator_refuses_another_networks_weights_as_a_whole(other, tmp_path):
     ev.rwlock.w_release()
     ev.set_weights(random_net(3, 3, 9, 1, 128, seed=3, norm="layer").state_dict())
     assert ev.version == version + 1
+
+
+def test_weights_that_are_no_tensors_are_refused_as_a_whole():
+    net = random_net(3, 3, 9, 1, 128, seed=1)
+    state = {k: t + 1 for k, t in net.state_dict().items()}
+    last = list(state)[-1]
+    for bad in (state[last].numpy(), None, 1.0):
+        with pytest.raises(RuntimeError, match="tensor"):
+            check_weights(net, dict(state, **{last: bad}))
