@@ -57,3 +57,16 @@ def test_on_the_cpu_a_trace_computes():
     with torch.no_grad():
         traced = torch.jit.trace(net, x)
         assert torch.allclose(traced(other), net(other), atol=1e-6) and not torch.allclose(traced(other), net(x), atol=1e-3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_networks_leave_the_operator_as_it_is(backend):
+    """torch.compile breaks its graph at the call and goes on behind it."""
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(8, 16), LayerNorm(16), torch.nn.Linear(16, 2)).cuda()
+    compiled = torch.compile(net, backend=backend)
+    for k in range(3):
+        x = torch.randn(3, 8, device="cuda")
+        grads = [torch.autograd.grad(f(x).square().sum(), list(net.parameters())) for f in (net, compiled)]
+        assert all(torch.allclose(a, b, rtol=1e-4, atol=1e-5) for a, b in zip(*grads))
